@@ -22,6 +22,7 @@
  *   nf_table_adam_step, nf_hash_encode_bwd_static, nf_hash_check_host : no counterpart (see their declarations)
  *   nf_revmlp_fwd / nf_revmlp_bwd : no counterpart in the reference (it has no
  *                             reversible MLP); same conventions as nf_mlp_*.
+ *   nf_rms_norm_*           : no counterpart (see their declarations)
  */
 #ifndef NF_CDNA4_H
 #define NF_CDNA4_H
@@ -286,6 +287,26 @@ int nf_revmlp_bwd_summed(const void* y, int64_t y_stride, const void* dy, int64_
                          void* dw1, void* db1, void* dw2, void* db2, int64_t rows, int half, int blocks, int act,
                          int dtype, int grad_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t nf_revmlp_bwd_workspace_bytes(int64_t rows, int half, int blocks);
+
+/* ---- wide layers: no counterpart in the reference, whose layers end at 64 channels ---- */
+
+/* Root-mean-square norm of rows.  h = x (+ residual), y = h / sqrt(mean(h^2) + eps) * weight, with float32 sums.
+ * x [rows, width] (x_dtype, row stride x_stride); residual NULL or rows of x's type or float32; weight NULL (ones) or [width] of any type;
+ * new_residual NULL or h rounded to the residual's type, rows of `width`; rstd NULL or the float32 factors that nf_rms_norm_bwd takes.
+ * scale NULL: y holds rows of x's type.  Otherwise y holds int8 rows and scale one float32 each: q = rint(v * (127 / a)), s = a / 127, a the
+ * largest magnitude of the row v; a row with an infinity or a NaN gets the scale NaN (and zeros), one below 2^-120 the scale zero. */
+int nf_rms_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const void* residual, int64_t residual_stride, int residual_dtype,
+                    const void* weight, int weight_dtype, void* y, float* scale, void* new_residual, float* rstd, int64_t rows, int64_t width,
+                    float eps, void* stream);
+
+/* Its gradients.  dy: of x's type; d_residual: NULL or the gradient that reached the new residual (h's type); h: the new residual, or x where
+ * there was none; dx [rows, width] of x's type, or NULL; dr: NULL (the residual's gradient is dx) or rows of h's type; dw: NULL or [width] of
+ * the weight's type, written, not added to, summed in a fixed order, with a workspace of nf_rms_norm_bwd_workspace_bytes() bytes.
+ * No rows: nothing is written, and dw must be NULL. */
+int64_t nf_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, const void* d_residual, int64_t d_residual_stride, const void* h,
+                    int64_t h_stride, int h_dtype, const float* rstd, const void* weight, int weight_dtype, void* dx, void* dr, void* dw,
+                    int64_t rows, int64_t width, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

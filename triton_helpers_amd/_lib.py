@@ -57,6 +57,9 @@ EXPORTS = (
     "nf_revmlp_bwd",
     "nf_revmlp_bwd_summed",
     "nf_revmlp_bwd_workspace_bytes",
+    "nf_rms_norm_fwd",
+    "nf_rms_norm_bwd",
+    "nf_rms_norm_bwd_workspace_bytes",
 )
 
 
@@ -143,6 +146,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nf_revmlp_bwd_summed.argtypes = [P, I64, P, I64, P, I64, P, I64, P, P, P, P, P, P, P, P, I64, I, I, I, I, I, P, I64, P]
     lib.nf_revmlp_bwd_workspace_bytes.restype = I64
     lib.nf_revmlp_bwd_workspace_bytes.argtypes = [I64, I, I]
+    lib.nf_rms_norm_fwd.restype = c_int
+    lib.nf_rms_norm_fwd.argtypes = [P, I64, I, P, I64, I, P, I, P, P, P, P, I64, I64, c_float, P]
+    lib.nf_rms_norm_bwd.restype = c_int
+    lib.nf_rms_norm_bwd.argtypes = [P, I64, I, P, I64, P, I64, I, P, P, I, P, P, P, I64, I64, P, I64, P]
+    lib.nf_rms_norm_bwd_workspace_bytes.restype = I64
+    lib.nf_rms_norm_bwd_workspace_bytes.argtypes = [I64, I64]
 
 
 def load() -> ctypes.CDLL:

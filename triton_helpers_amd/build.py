@@ -3,7 +3,7 @@
 ``python -m triton_helpers_amd.build`` cross-compiles every ``csrc/*.hip`` with
 ``hipcc --offload-arch=gfx950`` (no GPU needed) and links them into
 ``triton_helpers_amd/libnf_cdna4.so`` next to this file, then compiles the host side of the
-operators (``csrc/host_native.cpp``) into ``triton_helpers_amd/_native.so``.
+operators (``csrc/host_native.cpp``, ``csrc/host_wide.cpp``) into ``triton_helpers_amd/_native.so``.
 """
 from __future__ import annotations
 
@@ -15,7 +15,7 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
-from typing import List, Sequence
+from typing import List, Sequence, Tuple
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
@@ -60,6 +60,9 @@ SINGLE_READS = {"fused_mlp_bwd_roles.hip", "reversible_bwd.hip"}
 # spilled sum is read and written in every section, and the compiler has got one wrong in a kernel of this kind (it set the high half of a
 # 64-bit row counter aside in an accumulation register and never read it back).
 NO_SPILL = {"reversible_bwd.hip": "rev_bwd_k", "fused_mlp_bwd_roles.hip": "mlp_bwd_roles_k"}
+
+
+NATIVE_SOURCES = ("host_native.cpp", "host_wide.cpp")
 
 
 def _hipcc() -> str:
@@ -116,8 +119,9 @@ def sources() -> List[Path]:
     return sorted(CSRC.glob("*.hip"))
 
 
-def native_command(out: Path) -> List[str]:
-    """The operators' host side: a CPython module on torch's headers, linked to the kernel library beside it."""
+def native_commands(out: Path) -> Tuple[List[List[str]], List[str]]:
+    """The operators' host side: a CPython module on torch's headers, linked to the kernel library beside it (a command for each of its
+    files, and the one that links them)."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
@@ -126,10 +130,13 @@ def native_command(out: Path) -> List[str]:
         raise RuntimeError("a C++ compiler is required to build _native.so")
     rocm = Path(_hipcc()).resolve().parent.parent
     includes = [*include_paths(), str(rocm / "include"), sysconfig.get_paths()["include"]]
-    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *(f"-isystem{d}" for d in includes),
-            str(CSRC / "host_native.cpp"), "-o", str(out), f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", *(f"-L{d}" for d in library_paths()),
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *(f"-isystem{d}" for d in includes)]
+    objs = [str(BUILD_DIR / name.replace(".cpp", ".o")) for name in NATIVE_SOURCES]
+    compiles = [[cxx, *flags, "-c", str(CSRC / name), "-o", obj] for name, obj in zip(NATIVE_SOURCES, objs)]
+    link = [cxx, "-shared", *objs, "-o", str(out), f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", *(f"-L{d}" for d in library_paths()),
             "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    return compiles, link
 
 
 def build(verbose: bool = True, jobs: int = 8) -> Path:
@@ -150,14 +157,15 @@ def build(verbose: bool = True, jobs: int = 8) -> Path:
             flags += _feature(NO_MERGED_LDS)
         cmds.append(([hipcc, *flags, "-c", str(src), "-o", str(obj)], src))
         objs.append(obj)
+    tmp_native = NATIVE_PATH.with_suffix(".so.tmp")
+    host, link = native_commands(tmp_native)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        list(ex.map(lambda c: _compile(*c, verbose), cmds))
+        list(ex.map(lambda c: _compile(*c, verbose), [*cmds, *((c, CSRC / name) for c, name in zip(host, NATIVE_SOURCES))]))
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)], verbose)
     os.replace(tmp, LIB_PATH)
-    tmp = NATIVE_PATH.with_suffix(".so.tmp")
-    _run(native_command(tmp), verbose)
-    os.replace(tmp, NATIVE_PATH)
+    _run(link, verbose)
+    os.replace(tmp_native, NATIVE_PATH)
     return LIB_PATH
 
 

@@ -1,0 +1,200 @@
+// The host side of the wide layers (norm, 8-bit rows and products, the linear layer that keeps its input in 8 bits), in the manner of
+// host_native.cpp: a function for the plain case that returns None for everything else, and launch functions on checked arguments for
+// the Python functions that then take over.
+#include "host_common.h"
+
+namespace {
+
+bool float_type(const Tensor& t) { return code_of(t.scalar_type()) >= 0; }
+
+// ------------------------------------------------------------------------------------------------ norm
+struct Norm {
+  Tensor x, w, r;  // w, r: undefined without
+  float eps;
+  at::ScalarType stream_type() const { return r.defined() ? r.scalar_type() : x.scalar_type(); }
+};
+
+// An element type and sizes that the kernels take (the same conditions as the Python function's checks).
+bool norm_fits(const Norm& m) {
+  if (m.x.dim() < 1 || m.x.size(-1) < 1 || !float_type(m.x)) return false;
+  if (m.w.defined() && (!float_type(m.w) || m.w.dim() != 1 || m.w.size(0) != m.x.size(-1) || m.w.device() != m.x.device())) return false;
+  if (m.r.defined() && (m.r.sizes() != m.x.sizes() || m.r.device() != m.x.device() ||
+                        (m.r.scalar_type() != m.x.scalar_type() && m.r.scalar_type() != at::kFloat)))
+    return false;
+  return m.eps >= 0.0f;
+}
+
+struct NormOut {
+  Tensor y, scale, stream, rstd;
+};
+
+NormOut norm_forward(const Norm& m, bool eight, bool keep) {
+  const c10::DeviceGuard guard(m.x.device());
+  const int64_t width = m.x.size(-1);
+  const Rows x(m.x, width);
+  NormOut o;
+  o.y = at::empty(m.x.sizes(), eight ? m.x.options().dtype(at::kChar) : m.x.options());
+  if (eight) o.scale = at::empty(m.x.sizes().slice(0, m.x.dim() - 1), m.x.options().dtype(at::kFloat));
+  if (keep) o.rstd = at::empty({x.n}, m.x.options().dtype(at::kFloat));
+  std::optional<Rows> r;
+  if (m.r.defined()) {
+    r.emplace(m.r, width);
+    o.stream = at::empty(m.r.sizes(), m.r.options());
+  }
+  const Tensor w = contiguous(m.w);
+  check(nf_rms_norm_fwd(x.p, x.stride, code_of(m.x.scalar_type()), r ? r->p : nullptr, r ? r->stride : width, code_of(m.stream_type()), ptr(w),
+                        w.defined() ? code_of(w.scalar_type()) : NF_F32, o.y.data_ptr(), (float*)ptr(o.scale), ptr(o.stream), (float*)ptr(o.rstd), x.n,
+                        width, m.eps, stream_of(m.x)),
+        "nf_rms_norm_fwd");
+  return o;
+}
+
+// (dx, dw, dr).  h: the kept rows; dy, ds: the gradients of the output and of the new residual, either may be undefined.  `two`: dx and dr go
+// to leaves, which need a tensor each (autograd would copy a shared one).
+variable_list norm_backward(const Tensor& h, const Tensor& rstd, const Tensor& weight, at::ScalarType xt, Tensor dy, Tensor ds, bool residual,
+                            bool need_rows, bool need_w, bool two) {
+  const c10::DeviceGuard guard(h.device());
+  const int64_t width = h.size(-1);
+  const auto ht = h.scalar_type();
+  if (!dy.defined()) dy = at::zeros(h.sizes(), h.options().dtype(xt));
+  if (dy.scalar_type() != xt) dy = dy.to(xt);
+  if (ds.defined() && ds.scalar_type() != ht) ds = ds.to(ht);
+  const Rows rh(h, width), rd(dy, width);
+  std::optional<Rows> rs;
+  if (ds.defined()) rs.emplace(ds, width);
+  const Tensor w = contiguous(weight);
+  Tensor dx, dr, dw;
+  if (need_rows) {
+    dx = at::empty(h.sizes(), h.options().dtype(xt));
+    if (residual) dr = ht != xt || two ? at::empty(h.sizes(), h.options()) : dx;
+  }
+  need_w = need_w && w.defined();
+  if (need_w) dw = rh.n > 0 ? at::empty(w.sizes(), w.options()) : at::zeros(w.sizes(), w.options());
+  if (rh.n > 0 && (need_rows || need_w)) {
+    const int64_t bytes = need_w ? nf_rms_norm_bwd_workspace_bytes(rh.n, width) : 0;
+    const Tensor ws = scratch(bytes, h);
+    check(nf_rms_norm_bwd(rd.p, rd.stride, code_of(xt), rs ? rs->p : nullptr, rs ? rs->stride : width, rh.p, rh.stride, code_of(ht),
+                          rstd.data_ptr<float>(), ptr(w), w.defined() ? code_of(w.scalar_type()) : NF_F32, ptr(dx),
+                          dr.defined() && !dr.is_same(dx) ? dr.data_ptr() : nullptr, ptr(dw), rh.n, width, ptr(ws), bytes, stream_of(h)),
+          "nf_rms_norm_bwd");
+  }
+  return {dx, dw, dr};
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, std::optional<Tensor> w, std::optional<Tensor> r, double eps) {
+    const bool two = r && x.is_leaf() && r->is_leaf() && x.requires_grad() && r->requires_grad();
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Norm m{x, w.value_or(Tensor()), r.value_or(Tensor()), (float)eps};
+    NormOut o = norm_forward(m, false, true);
+    ctx->save_for_backward({r ? o.stream : x, o.rstd, m.w});
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    ctx->saved_data["residual"] = r.has_value();
+    ctx->saved_data["two"] = two;
+    ctx->set_materialize_grads(false);
+    return r ? variable_list{o.y, o.stream} : variable_list{o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const bool residual = ctx->saved_data["residual"].toBool();
+    // the engine counts the tensors that there are: an absent weight has no number
+    const bool weight = s[2].defined(), need_w = weight && ctx->needs_input_grad(1);
+    const bool need_rows = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(weight ? 2 : 1));
+    variable_list g = norm_backward(s[0], s[1], s[2], (at::ScalarType)ctx->saved_data["type"].toInt(), grads[0], residual ? grads[1] : Tensor(), residual,
+                                    need_rows, need_w, ctx->saved_data["two"].toBool());
+    return {g[0], g[1], g[2], Tensor()};
+  }
+};
+
+bool norm_args(PyObject* const* a, Norm* m) {
+  Tensor x;
+  std::optional<Tensor> w, r;
+  double eps;
+  if (modes_active() || !plain(a[0], &x) || !plain_or_none(a[1], &w) || !as_double(a[2], &eps) || !plain_or_none(a[3], &r)) return false;
+  *m = Norm{x, w.value_or(Tensor()), r.value_or(Tensor()), (float)eps};
+  return norm_fits(*m);
+}
+
+bool wants_grad(const Norm& m) {
+  return at::GradMode::is_enabled() && (m.x.requires_grad() || (m.w.defined() && m.w.requires_grad()) || (m.r.defined() && m.r.requires_grad()));
+}
+
+// rms_norm(x, weight, eps, residual): y, or (y, new residual)
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  Norm m;
+  if (!norm_args(a, &m)) Py_RETURN_NONE;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release release;
+    if (wants_grad(m)) {
+      const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+      out = RmsNorm::apply(m.x, opt(m.w), opt(m.r), (double)m.eps);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      NormOut o = norm_forward(m, false, false);
+      out = m.r.defined() ? variable_list{o.y, o.stream} : variable_list{o.y};
+    }
+  }
+  return out.size() == 1 ? wrap(out[0]) : wrap_list(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_int8(x, weight, eps, residual): (q, scale), or (q, scale, new residual)
+PyObject* rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  Norm m;
+  if (!norm_args(a, &m) || wants_grad(m)) Py_RETURN_NONE;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    NormOut o = norm_forward(m, true, false);
+    out = {o.y, o.scale};
+    if (m.r.defined()) out.push_back(o.stream);
+  }
+  return wrap_list(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_launch_forward(x, weight, eps, residual, eight) on checked arguments: (y, scale or None, new residual or None, rstd or None)
+PyObject* rms_norm_launch_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(5);
+  double eps;
+  TORCH_CHECK(as_double(a[2], &eps), "eps expected");
+  const Norm m{tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[3]), (float)eps};
+  const bool eight = a[4] == Py_True;
+  NormOut o;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    o = norm_forward(m, eight, !eight);
+  }
+  return wrap_list({o.y, o.scale, o.stream, o.rstd});
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_launch_backward(h, rstd, weight, like, dy, d_residual, residual, need_rows, need_w): (dx, dw, dr); `like`: a tensor of x's type
+PyObject* rms_norm_launch_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(9);
+  const Tensor h = tensor_arg(a[0]), rstd = tensor_arg(a[1]), w = tensor_arg(a[2]), like = tensor_arg(a[3]), dy = tensor_arg(a[4]), ds = tensor_arg(a[5]);
+  const bool residual = a[6] == Py_True, need_rows = a[7] == Py_True, need_w = a[8] == Py_True;
+  variable_list g;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    g = norm_backward(h, rstd, w, like.scalar_type(), dy, ds, residual, need_rows, need_w, residual);
+  }
+  return wrap_list(g);
+  END_HANDLE_TH_ERRORS
+}
+
+}  // namespace
+
+PyMethodDef wide_methods[] = {ENTRY(rms_norm), ENTRY(rms_norm_int8), ENTRY(rms_norm_launch_forward), ENTRY(rms_norm_launch_backward),
+                              {nullptr, nullptr, 0, nullptr}};

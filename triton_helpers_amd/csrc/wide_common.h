@@ -1,0 +1,154 @@
+// What the kernels of the wide layers (norm, 8-bit rows, products) share: eight values of a row at a time, sums over the threads of a row,
+// the 8-bit form of a row, and the activations.
+#pragma once
+
+#include <type_traits>
+
+#include "mlp_tile.h"
+#include "nf_common.h"
+
+namespace nf {
+
+// Eight consecutive values from any address of their type: one or two 16-byte loads (this chip takes them off 16-byte boundaries), or the n
+// that are left of a row, and zeros.
+template <typename T>
+__device__ __forceinline__ void load8(const typename T::storage* p, int n, float (&v)[8]) {
+  typename T::storage raw[8];
+  if (n >= 8) {
+    __builtin_memcpy(raw, p, sizeof raw);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : typename T::storage(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = T::to_f32(raw[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(typename T::storage* p, int n, const float (&v)[8]) {
+  typename T::storage raw[8];
+  if constexpr (std::is_same<T, F32>::value) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = v[i];
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = T::pack(v[2 * i], v[2 * i + 1]);
+    __builtin_memcpy(raw, w, sizeof raw);
+  }
+  if (n >= 8) {
+    __builtin_memcpy(p, raw, sizeof raw);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = raw[i];
+  }
+}
+// eight values of a type that is known at run time only (a norm's weight; the branch is the same for every thread)
+__device__ __forceinline__ void load8_any(const void* p, int64_t at, int n, int dt, float (&v)[8]) {
+  if (dt == NF_F32) load8<F32>((const float*)p + at, n, v);
+  else if (dt == NF_F16) load8<F16>((const uint16_t*)p + at, n, v);
+  else load8<BF16>((const uint16_t*)p + at, n, v);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t at, int dt, float v) {
+  if (dt == NF_F32) ((float*)p)[at] = v;
+  else ((uint16_t*)p)[at] = dt == NF_F16 ? F16::from_f32(v) : BF16::from_f32(v);
+}
+__device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&q)[8]) {
+  int8_t raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) raw[i] = (int8_t)(int)q[i];
+  if (n >= 8) {
+    __builtin_memcpy(p, raw, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = raw[i];
+  }
+}
+
+// ---- over the T threads of a row (T = 64: a wave; else the whole workgroup) -----------------
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t u = __shfl_xor(v, o);
+    v = v > u ? v : u;
+  }
+  return v;
+}
+// `shared`: T / 64 values of its own for every call between two barriers
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+  v = wave_sum(v);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) v += shared[i];
+  }
+  return v;
+}
+template <int T>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
+  v = wave_max(v);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) v = v > shared[i] ? v : shared[i];
+  }
+  return v;
+}
+
+// ---- the 8-bit form of a row ----------------------------------------------------------------
+// q = rint(v * (127 / a)), s = a / 127, a the largest magnitude.  The magnitudes are compared as bit patterns, in which infinities come
+// behind every number and NaN behind them: a row that holds either has no 8-bit form, its scale becomes NaN and with it whatever is
+// made of the row.  A row of magnitudes below 2^-120, whose 127 / a would leave float32, counts as zeros.
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+struct EightBit {
+  float scale, inverse;
+};
+__device__ __forceinline__ EightBit eight_bit(uint32_t largest) {
+  const float a = __uint_as_float(largest);
+  if (largest >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.0f};
+  if (a < 7.5231638e-37f) return {0.0f, 0.0f};
+  return {a / 127.0f, 127.0f / a};
+}
+// of a row with a scale; NaN and infinities (inverse = 0) become zeros
+__device__ __forceinline__ float quantized(float v, EightBit e) { return e.inverse == 0.0f ? 0.0f : rintf(v * e.inverse); }
+
+// ---- activations ------------------------------------------------------------------------------
+// As act_fwd / act_grad, which are made for 16-bit results, but for a GELU that is right to 1.5e-7, and a NaN stays one.
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == NF_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  else if constexpr (ACT == NF_ACT_RELU2) return z < 0.0f ? 0.0f : z * z;
+  else if constexpr (ACT == NF_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  else if constexpr (ACT == NF_ACT_GELU) {
+    float pdf;
+    return z * normal_cdf_pdf(z, &pdf);
+  } else return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == NF_ACT_RELU) return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
+  else if constexpr (ACT == NF_ACT_RELU2) return z <= 0.0f ? 0.0f : 2.0f * z;
+  else if constexpr (ACT == NF_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    return s * (z * (1.0f - s) + 1.0f);
+  } else if constexpr (ACT == NF_ACT_GELU) {
+    float pdf;
+    const float cdf = normal_cdf_pdf(z, &pdf);
+    return cdf + z * pdf;
+  } else return 1.0f;
+}
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+}  // namespace nf
