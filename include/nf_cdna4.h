@@ -22,7 +22,7 @@
  *   nf_table_adam_step, nf_hash_encode_bwd_static, nf_hash_check_host : no counterpart (see their declarations)
  *   nf_revmlp_fwd / nf_revmlp_bwd : no counterpart in the reference (it has no
  *                             reversible MLP); same conventions as nf_mlp_*.
- *   nf_rms_norm_*           : no counterpart (see their declarations)
+ *   nf_rms_norm_*, nf_quantize_rows, nf_int8_linear : no counterpart (see their declarations)
  */
 #ifndef NF_CDNA4_H
 #define NF_CDNA4_H
@@ -307,6 +307,21 @@ int64_t nf_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
 int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, const void* d_residual, int64_t d_residual_stride, const void* h,
                     int64_t h_stride, int h_dtype, const float* rstd, const void* weight, int weight_dtype, void* dx, void* dr, void* dw,
                     int64_t rows, int64_t width, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows as int8 with one float32 scale each: q = rint(x * (127 / a)), s = a / 127, a the largest magnitude of the row (as nf_rms_norm_fwd's 8-bit
+ * rows).  q [rows, width] without gaps.  h: NULL, or act(x) in x's type, rows h_stride values apart, h_stride the width or the next multiple
+ * of 8 (the values in between become zeros). */
+int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int8_t* q, float* scale, void* h, int64_t h_stride, int act, int64_t rows,
+                     int64_t width, void* stream);
+
+/* y[m, n] = act(scale[m] * w_scale[n] * sum_k q[m, k] * w[n, k] + bias[n]) for int8 q [rows, k] and w [n, k] (row strides in values, at least k), exact
+ * 32-bit integer sums (k at most 131071), float32 behind them, rounded once to y's type.  bias: NULL or [n] of any type.  Up to 64 rows
+ * need no workspace; nf_int8_linear_workspace_bytes() says what the call with these pointers and strides needs, 16-byte aligned (copies of
+ * rows off 16-byte boundaries, partial sums where the summed dimension is split). */
+int64_t nf_int8_linear_workspace_bytes(const int8_t* q, int64_t q_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k);
+int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const int8_t* w, int64_t w_stride, const float* w_scale, const void* bias,
+                   int bias_dtype, void* y, int64_t y_stride, int y_dtype, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
+                   int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -73,3 +73,68 @@ def test_norm_arguments():
             f(x.double(), None)
         with pytest.raises(NotImplementedError, match="weight"):
             f(x, torch.ones(64, dtype=torch.int32))
+
+
+def test_product_entry_points():
+    lib = _lib.load()
+
+    def product(q=16, qs=64, s=16, w=16, ws=64, t=16, y=16, ys=48, ydt=BF, bdt=F32, rows=4, n=48, k=64, act=0, work=None, size=0):
+        return lib.nf_int8_linear(q, qs, s, w, ws, t, None, bdt, y, ys, ydt, rows, n, k, act, work, size, None)
+
+    refused(product(ydt=9), -1, b"dtype")
+    refused(product(act=5), -1, b"activation")
+    refused(product(rows=-1), -1, b"rows")
+    refused(product(n=0), -1, b"n=0")
+    refused(product(k=0), -1, b"k=0")
+    refused(product(k=131072, qs=131072, ws=131072), -2, b"131071")
+    refused(product(s=None), -1, b"NULL")
+    refused(product(qs=63), -1, b"stride")
+    refused(product(ws=63), -1, b"stride")
+    refused(product(ys=47), -1, b"stride")
+    assert product(rows=0, q=None) == 0
+    # few rows, and whole pieces in one run of tiles, need nothing; rows off 16-byte boundaries a copy; a split sum its parts
+    size = lib.nf_int8_linear_workspace_bytes
+    assert size(16, 64, 16, 64, 64, 48, 64) == 0 and size(1, 63, 3, 63, 64, 48, 63) == 0
+    assert size(16, 64, 16, 64, 65, 48, 64) == 0
+    assert size(1, 64, 16, 64, 65, 48, 64) >= 65 * 64 and size(16, 64, 17, 64, 65, 48, 64) >= 48 * 64
+    assert size(16, 63, 16, 64, 65, 48, 63) >= (65 + 48) * 64
+    need = size(16, 8192, 16, 8192, 65, 48, 8192)
+    assert need >= 2 * 65 * 48 * 4
+    refused(product(qs=8192, ws=8192, rows=65, k=8192, work=16, size=need - 1), -1, b"workspace")
+    refused(product(qs=8192, ws=8192, rows=65, k=8192, work=24, size=need), -1, b"workspace")
+
+    def quantize(x=16, xs=64, dt=BF, q=16, s=16, h=None, hs=64, act=0, rows=4, width=64):
+        return lib.nf_quantize_rows(x, xs, dt, q, s, h, hs, act, rows, width, None)
+
+    refused(quantize(dt=3), -1, b"dtype")
+    refused(quantize(act=-1), -1, b"activation")
+    refused(quantize(rows=2**31), -1, b"rows")
+    refused(quantize(width=0), -1, b"width")
+    refused(quantize(h=16, hs=65), -1, b"h_stride")
+    refused(quantize(q=None), -1, b"NULL")
+    refused(quantize(xs=63), -1, b"stride")
+    assert quantize(rows=0) == 0
+
+
+def test_product_arguments():
+    from triton_helpers_amd.layers.int8_linear import int8_linear, quantize_rows
+
+    q, s = torch.zeros(4, 64, dtype=torch.int8), torch.ones(4)
+    w, t = torch.zeros(48, 64, dtype=torch.int8), torch.ones(48)
+    with pytest.raises(AssertionError, match="GPU"):
+        int8_linear(q, s, w, t)
+    for bad, word in (((q.float(), s, w, t), "q must be int8"), ((q, s.half(), w, t), "scale must be float32"), ((q, s, w[:, :63], t), "w must be"),
+                      ((q, s[:3], w, t), "scale must have"), ((q, s, w, t[:3]), "w_scale must be"), ((q, s, w, t, torch.ones(47)), "bias must be"),
+                      ((q, s, w, t, None, "tanh"), "activation"), ((q, s, w.int(), t), "w must be int8"), ((q[:, :0], s, w[:, :0], t), "last dimension")):
+        with pytest.raises(AssertionError, match=word):
+            int8_linear(*bad)
+    with pytest.raises(NotImplementedError):
+        int8_linear(q, s, w, t, dtype=torch.float64)
+    with pytest.raises(NotImplementedError):
+        int8_linear(q, s, w, t, torch.ones(48, dtype=torch.float64))
+    with pytest.raises(AssertionError, match="GPU"):
+        quantize_rows(torch.randn(4, 64))
+    with pytest.raises(NotImplementedError, match="int8"):
+        quantize_rows(q)
+    with pytest.raises(AssertionError, match="last dimension"):
+        quantize_rows(torch.randn(4, 0))

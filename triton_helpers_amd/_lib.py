@@ -60,6 +60,9 @@ EXPORTS = (
     "nf_rms_norm_fwd",
     "nf_rms_norm_bwd",
     "nf_rms_norm_bwd_workspace_bytes",
+    "nf_quantize_rows",
+    "nf_int8_linear",
+    "nf_int8_linear_workspace_bytes",
 )
 
 
@@ -152,6 +155,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nf_rms_norm_bwd.argtypes = [P, I64, I, P, I64, P, I64, I, P, P, I, P, P, P, I64, I64, P, I64, P]
     lib.nf_rms_norm_bwd_workspace_bytes.restype = I64
     lib.nf_rms_norm_bwd_workspace_bytes.argtypes = [I64, I64]
+    lib.nf_quantize_rows.restype = c_int
+    lib.nf_quantize_rows.argtypes = [P, I64, I, P, P, P, I64, I, I64, I64, P]
+    lib.nf_int8_linear.restype = c_int
+    lib.nf_int8_linear.argtypes = [P, I64, P, P, I64, P, P, I, P, I64, I, I64, I64, I64, I, P, I64, P]
+    lib.nf_int8_linear_workspace_bytes.restype = I64
+    lib.nf_int8_linear_workspace_bytes.argtypes = [P, I64, P, I64, I64, I64, I64]
 
 
 def load() -> ctypes.CDLL:

@@ -194,7 +194,131 @@ PyObject* rms_norm_launch_backward(PyObject*, PyObject* const* a, Py_ssize_t n) 
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ 8-bit rows and products
+// (q, scale)
+variable_list quantize(const Tensor& x) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t width = x.size(-1);
+  const Rows r(x, width);
+  const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar));
+  const Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  check(nf_quantize_rows(r.p, r.stride, code_of(x.scalar_type()), (int8_t*)q.data_ptr(), (float*)scale.data_ptr(), nullptr, width, NF_ACT_NONE, r.n,
+                         width, stream_of(x)),
+        "nf_quantize_rows");
+  return {q, scale};
+}
+
+struct Int8 {
+  Tensor q, scale, w, w_scale, bias;
+  int act;
+  at::ScalarType type;
+};
+
+bool int8_fits(const Int8& m) {
+  if (m.q.dim() < 1 || m.w.dim() != 2 || m.q.size(-1) < 1 || m.q.size(-1) > 131071 || m.w.size(0) < 1 || m.w.size(1) != m.q.size(-1)) return false;
+  if (m.q.scalar_type() != at::kChar || m.w.scalar_type() != at::kChar || m.scale.scalar_type() != at::kFloat || m.w_scale.scalar_type() != at::kFloat)
+    return false;
+  if (m.scale.sizes() != m.q.sizes().slice(0, m.q.dim() - 1) || m.w_scale.dim() != 1 || m.w_scale.size(0) != m.w.size(0)) return false;
+  if (m.bias.defined() && (!float_type(m.bias) || m.bias.dim() != 1 || m.bias.size(0) != m.w.size(0))) return false;
+  for (const Tensor* t : {&m.scale, &m.w, &m.w_scale, &m.bias})
+    if (t->defined() && t->device() != m.q.device()) return false;
+  return code_of(m.type) >= 0;
+}
+
+Tensor int8_forward(const Int8& m) {
+  const c10::DeviceGuard guard(m.q.device());
+  const int64_t k = m.q.size(-1), n = m.w.size(0);
+  const Rows q(m.q, k), w(m.w, k);
+  c10::SmallVector<int64_t, 5> shape(m.q.sizes().begin(), m.q.sizes().end());
+  shape.back() = n;
+  const Tensor y = at::empty(shape, m.q.options().dtype(m.type)), scale = contiguous(m.scale), w_scale = contiguous(m.w_scale), bias = contiguous(m.bias);
+  const auto* qp = (const int8_t*)q.p;
+  const auto* wp = (const int8_t*)w.p;
+  const int64_t bytes = nf_int8_linear_workspace_bytes(qp, q.stride, wp, w.stride, q.n, n, k);
+  const Tensor ws = scratch(bytes, m.q);
+  check(nf_int8_linear(qp, q.stride, (const float*)scale.data_ptr(), wp, w.stride, (const float*)w_scale.data_ptr(), ptr(bias),
+                       bias.defined() ? code_of(bias.scalar_type()) : NF_F32, y.data_ptr(), n, code_of(m.type), q.n, n, k, m.act, ptr(ws), bytes,
+                       stream_of(m.q)),
+        "nf_int8_linear");
+  return y;
+}
+
+bool needs_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.defined() && t.requires_grad(); }
+
+// quantize_rows(x): (q, scale)
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(1);
+  Tensor x;
+  if (modes_active() || !plain(a[0], &x) || x.dim() < 1 || x.size(-1) < 1 || !float_type(x) || needs_grad(x)) Py_RETURN_NONE;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = quantize(x);
+  }
+  return wrap_list(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_linear(q, scale, w, w_scale, bias, activation, code of the result's type)
+PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(7);
+  Int8 m;
+  std::optional<Tensor> bias;
+  int64_t type;
+  m.act = activation(a[5], true);
+  if (modes_active() || m.act < 0 || !plain(a[0], &m.q) || !plain(a[1], &m.scale) || !plain(a[2], &m.w) || !plain(a[3], &m.w_scale) ||
+      !plain_or_none(a[4], &bias) || !as_int(a[6], &type) || type < NF_F32 || type > NF_BF16)
+    Py_RETURN_NONE;
+  m.bias = bias.value_or(Tensor());
+  m.type = type == NF_F32 ? at::kFloat : type == NF_F16 ? at::kHalf : at::kBFloat16;
+  if (!int8_fits(m) || needs_grad(m.scale) || needs_grad(m.w_scale) || needs_grad(m.bias)) Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    y = int8_forward(m);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// quantize_rows_launch(x), int8_linear_launch(q, scale, w, w_scale, bias, activation code, type code): on checked arguments
+PyObject* quantize_rows_launch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(1);
+  const Tensor x = tensor_arg(a[0]);
+  variable_list out;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = quantize(x);
+  }
+  return wrap_list(out);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* int8_linear_launch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(7);
+  int64_t act, type;
+  TORCH_CHECK(as_int(a[5], &act) && as_int(a[6], &type), "codes expected");
+  const Int8 m{tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]), tensor_arg(a[3]), tensor_arg(a[4]), (int)act,
+               type == NF_F32 ? at::kFloat : type == NF_F16 ? at::kHalf : at::kBFloat16};
+  Tensor y;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    y = int8_forward(m);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 }  // namespace
 
 PyMethodDef wide_methods[] = {ENTRY(rms_norm), ENTRY(rms_norm_int8), ENTRY(rms_norm_launch_forward), ENTRY(rms_norm_launch_backward),
+                              ENTRY(quantize_rows), ENTRY(quantize_rows_launch), ENTRY(int8_linear), ENTRY(int8_linear_launch),
                               {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,314 @@
+// Product of 8-bit rows and 8-bit weight rows with a scale for each row of either, bias and activation behind it:
+//
+//   y[m, n] = act(s[m] t[n] sum_k q[m, k] w[n, k] + b[n])
+//
+// The sums are exact: 32-bit integers up to 131071 products of at most 2^14.
+//
+// Up to 64 rows the time is that of reading the weights once: int8_few_rows_k, no LDS for the operands, the summed dimension split over the waves of
+// a workgroup.  Beyond, tiles on the 8-bit matrix instructions (gemm_tile.h); where the tiles are too few for the chip, the summed
+// dimension is split over workgroups, whose integer sums a second kernel adds up (integers: any order gives the same bits).
+#include "gemm_tile.h"
+
+namespace nf {
+
+struct Epilogue {
+  const float *s, *t;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int bias_dt, y_dt, act, m, n;
+};
+
+template <int ACT, typename YT>
+__device__ __forceinline__ void put4(const Epilogue& e, int m, int n, const int (&sum)[4], float s) {
+  const int left = e.n - n;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = i < left ? n + i : n;
+    const float z = (float)sum[i] * (s * e.t[c]);
+    v[i] = act_value<ACT>(e.bias == nullptr ? z : z + load_as_f32(e.bias, c, e.bias_dt));
+  }
+  auto* o = (typename YT::storage*)e.y + (int64_t)m * e.ldy + n;
+  if constexpr (std::is_same<YT, F32>::value) {
+    if (left >= 4) __builtin_memcpy(o, v, 16);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = v[i];
+  } else {
+    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
+    if (left >= 4) __builtin_memcpy(o, w, 8);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+  }
+}
+
+// body(activation, type of y) under one branch that is the same for every thread
+template <typename Body>
+__device__ __forceinline__ void with_epilogue(const Epilogue& e, Body&& body) {
+  with_act(e.act, [&](auto act_c) {
+    if (e.y_dt == NF_F32) body(act_c, F32{});
+    else if (e.y_dt == NF_F16) body(act_c, F16{});
+    else body(act_c, BF16{});
+  });
+}
+
+// ---- few rows -----------------------------------------------------------------------------------
+struct FewRows {
+  const char *q, *w;
+  int64_t ldq, ldw;
+  int k;
+  Epilogue e;
+};
+
+// 16 bytes of a row from any address; bytes beyond the row's end are zeros
+__device__ __forceinline__ i32x4_t load16(const char* row, int at, int end) {
+  i32x4_t v = {0, 0, 0, 0};
+  if (at + 16 <= end) {
+    __builtin_memcpy(&v, row + at, 16);
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+      if (at + i < end) w[i / 4] |= (uint32_t)(uint8_t)row[at + i] << (i % 4 * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (int)w[i];
+  }
+  return v;
+}
+
+// 16 MT rows and 16 NT columns a workgroup.  A wave's unit is 256 bytes of each row, of which the four groups of sixteen lanes take 64 bytes each
+// (whole cache lines of the weights in four loads); the units are dealt to the W waves in turn, and their sums meet in LDS.
+template <int MT, int NT, int W>
+__global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
+  __shared__ int part[W][MT * NT][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NT;
+  const char *wp[NT], *qp[MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + 16 * j + r;
+    wp[j] = a.w + (int64_t)(n < a.e.n ? n : a.e.n - 1) * a.ldw;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = 16 * i + r;
+    qp[i] = a.q + (int64_t)(m < a.e.m ? m : a.e.m - 1) * a.ldq;
+  }
+  i32x4_t acc[MT][NT] = {};
+  const auto unit = [&](int u, auto whole_c) {
+    const int k = u * 256 + g * 64;
+    i32x4_t fw[NT][4], fq[MT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&fw[j][s], wp[j] + k + 16 * s, 16);
+        else fw[j][s] = load16(wp[j], k + 16 * s, a.k);
+      }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&fq[i][s], qp[i] + k + 16 * s, 16);
+        else fq[i][s] = load16(qp[i], k + 16 * s, a.k);
+      }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<I8>::run(fw[j][s], fq[i][s], acc[i][j]);
+  };
+  const int whole = a.k / 256;
+  for (int u = wave; u < whole; u += W) unit(u, Int<1>{});
+  if (whole * 256 < a.k && whole % W == wave) unit(whole, Int<0>{});
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) part[wave][i * NT + j][c][lane] = acc[i][j][c];
+  __syncthreads();
+  // a thread adds up four neighbouring columns of a row: lane and numbers as the matrix instruction left them
+  for (int at = threadIdx.x; at < MT * NT * 64; at += 64 * W) {
+    const int j = at % (4 * NT), m = at / (4 * NT);  // four columns 4 j, row m
+    const int from = (j & 3) * 16 + (m & 15), tile = (m >> 4) * NT + (j >> 2);
+    const int n = n0 + 4 * j;
+    if (m >= a.e.m || n >= a.e.n) continue;
+    int sum[4] = {};
+#pragma unroll
+    for (int v = 0; v < W; ++v)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] += part[v][tile][c][from];
+    const float s = a.e.s[m];
+    with_epilogue(a.e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s); });
+  }
+}
+
+// ---- tiles --------------------------------------------------------------------------------------
+template <typename G, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogue e, int* slots) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
+  i32x4_t acc[G::FM][G::FN] = {};
+  const Tile t = tile_of(g, blockIdx.x);
+  G::run(g, t, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = t.m * BM + wave / WN * (BM / WM) + (lane & 15), n0 = t.n * BN + wave % WN * (BN / WN) + (lane >> 4) * 4;
+  if (slots != nullptr) {  // [split][m][n rounded up to 4]
+    const int64_t ld = (g.n + 3) / 4 * 4;
+    int* o = slots + (int64_t)t.split * g.m * ld;
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) {
+        const int m = m0 + 16 * i, n = n0 + 16 * j;
+        if (m < g.m && n < g.n) *(i32x4_t*)(o + (int64_t)m * ld + n) = acc[i][j];
+      }
+    return;
+  }
+  with_epilogue(e, [&](auto act_c, auto y_c) {
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i) {
+      const int m = m0 + 16 * i;
+      if (m >= g.m) continue;
+      const float s = e.s[m];
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) {
+        const int n = n0 + 16 * j;
+        const int sum[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (n < g.n) put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s);
+      }
+    }
+  });
+}
+
+__global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, Epilogue e) {
+  const int64_t quads = (e.n + 3) / 4, ld = quads * 4, each = (int64_t)e.m * ld;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= e.m * quads) return;
+  const int m = (int)(at / quads), n = (int)(at % quads) * 4;
+  i32x4_t v = {0, 0, 0, 0};
+  for (int k = 0; k < splits; ++k) v += *(const i32x4_t*)(slots + k * each + (int64_t)m * ld + n);
+  const int sum[4] = {v[0], v[1], v[2], v[3]};
+  const float s = e.s[m];
+  with_epilogue(e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s); });
+}
+
+// rows copied to 16-byte boundaries and filled up with zeros, 16 bytes a thread
+__global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld, int bytes, char* to, int64_t rows) {
+  const int pieces = (bytes + 15) / 16;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const int64_t row = at / pieces;
+  const int k = (int)(at % pieces) * 16;
+  *(i32x4_t*)(to + row * pieces * 16 + k) = load16(from + row * ld, k, bytes);
+}
+
+struct Plan {
+  bool few;
+  int bm, splits, split_steps;
+  bool pack_q, pack_w;
+  int64_t q_bytes, w_bytes, slot_bytes;
+  int64_t total() const { return q_bytes + w_bytes + slot_bytes; }
+};
+
+inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
+inline bool rows_fit(const void* p, int64_t ld, int64_t k) { return k % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
+
+constexpr int FEW_ROWS = 64;
+
+Plan plan(const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k) {
+  Plan p{};
+  p.few = m <= FEW_ROWS;
+  if (p.few) return p;
+  p.pack_q = !rows_fit(q, ldq, k);
+  p.pack_w = !rows_fit(w, ldw, k);
+  if (p.pack_q) p.q_bytes = round_up(m * round_up(k, 16), 256);
+  if (p.pack_w) p.w_bytes = round_up(n * round_up(k, 16), 256);
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
+  p.bm = big >= 192 ? 256 : 128;
+  const int64_t tiles = p.bm == 256 ? big : small, steps = (k + STEP - 1) / STEP;
+  int64_t splits = p.bm == 256 ? 1 : 512 / tiles;
+  if (splits > steps / 8) splits = steps / 8;
+  if (splits < 1) splits = 1;
+  p.split_steps = (int)((steps + splits - 1) / splits);
+  p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
+  if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 4) * 4, 256);
+  return p;
+}
+
+template <int BM, int BN, int WM, int WN, int S>
+int tile_launch(GemmArgs g, const Epilogue& e, int* slots, hipStream_t s) {
+  typedef Gemm<I8, BM, BN, WM, WN, S> G;
+  g.tiles_m = (g.m + BM - 1) / BM;
+  g.tiles_n = (g.n + BN - 1) / BN;
+  hipLaunchKernelGGL((int8_tile_k<G, BM, BN, WM, WN>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e, slots);
+  return check_launch("int8_linear");
+}
+
+}  // namespace nf
+
+using namespace nf;
+
+extern "C" int64_t nf_int8_linear_workspace_bytes(const int8_t* q, int64_t q_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k) {
+  if (rows <= 0 || n <= 0 || k <= 0 || rows >= (1ll << 31) || n >= (1ll << 31) || k > 131071) return 0;
+  return plan(q, q_stride, w, w_stride, rows, n, k).total();
+}
+
+extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const int8_t* w, int64_t w_stride, const float* w_scale,
+                              const void* bias, int bias_dtype, void* y, int64_t y_stride, int y_dtype, int64_t rows, int64_t n, int64_t k, int act,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  NF_REQUIRE(dtype_ok(y_dtype) && dtype_ok(bias_dtype), NF_EINVAL, "unknown dtype code");
+  NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
+  NF_REQUIRE(rows >= 0 && rows < (1ll << 31), NF_EINVAL, "rows=%lld outside 0..2^31-1", (long long)rows);
+  NF_REQUIRE(n >= 1 && n < (1ll << 31) - 256, NF_EINVAL, "n=%lld outside 1..2^31-257", (long long)n);
+  NF_REQUIRE(k >= 1, NF_EINVAL, "k=%lld below 1", (long long)k);
+  NF_REQUIRE(k <= 131071, NF_EUNSUPPORTED, "k=%lld: more than 131071 products leave a 32-bit integer sum", (long long)k);
+  if (rows == 0) return 0;
+  NF_REQUIRE(q && scale && w && w_scale && y, NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE((rows == 1 || (q_stride >= k && y_stride >= n)) && (n == 1 || w_stride >= k), NF_EINVAL, "row stride below the row's length");
+  const Plan p = plan(q, q_stride, w, w_stride, rows, n, k);
+  NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
+             "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
+  hipStream_t s = (hipStream_t)stream;
+  const Epilogue e{scale, w_scale, bias, y, y_stride, bias_dtype, y_dtype, act, (int)rows, (int)n};
+  if (p.few) {
+    const FewRows a{(const char*)q, (const char*)w, q_stride, w_stride, (int)k, e};
+    const auto go = [&](auto mt, auto nt) {
+      constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
+      hipLaunchKernelGGL((int8_few_rows_k<MT, NT, 8>), dim3((unsigned)((n + 16 * NT - 1) / (16 * NT))), dim3(512), 0, s, a);
+    };
+    if (rows <= 16) go(Int<1>{}, Int<1>{});
+    else if (rows <= 32) go(Int<2>{}, Int<1>{});
+    else go(Int<4>{}, Int<2>{});
+    return check_launch("int8_linear");
+  }
+  char* ws = (char*)workspace;
+  const char *a = (const char*)q, *b = (const char*)w;
+  int64_t lda = q_stride, ldb = w_stride;
+  const auto pack = [&](const char* from, int64_t ld, int64_t count, char* to) {
+    const int64_t pieces = (k + 15) / 16;
+    hipLaunchKernelGGL(pack_rows_k, dim3((unsigned)((count * pieces + 255) / 256)), dim3(256), 0, s, from, ld, (int)k, to, count);
+    return check_launch("pack_rows");
+  };
+  if (p.pack_q) {
+    if (const int rc = pack(a, lda, rows, ws)) return rc;
+    a = ws;
+    lda = round_up(k, 16);
+  }
+  if (p.pack_w) {
+    if (const int rc = pack(b, ldb, n, ws + p.q_bytes)) return rc;
+    b = ws + p.q_bytes;
+    ldb = round_up(k, 16);
+  }
+  const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)round_up(k, 16), 0, 0, p.splits, p.split_steps};
+  int* slots = p.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
+  const int rc = p.bm == 256 ? tile_launch<256, 256, 2, 4, 4>(g, e, slots, s) : tile_launch<128, 128, 2, 2, 4>(g, e, slots, s);
+  if (rc != 0 || slots == nullptr) return rc;
+  hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
+  return check_launch("int8_sum");
+}
