@@ -22,7 +22,7 @@
  *   nf_table_adam_step, nf_hash_encode_bwd_static, nf_hash_check_host : no counterpart (see their declarations)
  *   nf_revmlp_fwd / nf_revmlp_bwd : no counterpart in the reference (it has no
  *                             reversible MLP); same conventions as nf_mlp_*.
- *   nf_rms_norm_*, nf_quantize_rows, nf_int8_linear : no counterpart (see their declarations)
+ *   nf_rms_norm_*, nf_quantize_rows, nf_int8_linear, nf_linear_keep_* : no counterpart (see their declarations)
  */
 #ifndef NF_CDNA4_H
 #define NF_CDNA4_H
@@ -309,7 +309,7 @@ int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, const void* 
                     int64_t rows, int64_t width, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Rows as int8 with one float32 scale each: q = rint(x * (127 / a)), s = a / 127, a the largest magnitude of the row (as nf_rms_norm_fwd's 8-bit
- * rows).  q [rows, width] without gaps.  h: NULL, or act(x) in x's type, rows h_stride values apart, h_stride the width or the next multiple
+ * rows).  q [rows, width] without gaps, or NULL where h alone is wanted.  h: NULL, or act(x) in x's type, rows h_stride values apart, h_stride the width or the next multiple
  * of 8 (the values in between become zeros). */
 int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int8_t* q, float* scale, void* h, int64_t h_stride, int act, int64_t rows,
                      int64_t width, void* stream);
@@ -322,6 +322,23 @@ int64_t nf_int8_linear_workspace_bytes(const int8_t* q, int64_t q_stride, const 
 int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const int8_t* w, int64_t w_stride, const float* w_scale, const void* bias,
                    int bias_dtype, void* y, int64_t y_stride, int y_dtype, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
                    int64_t workspace_bytes, void* stream);
+
+/* A linear layer behind an activation that keeps its input as 8-bit rows for the backward, float16 or bfloat16 rows and weights.
+ *   forward   y[m, n] = sum_k act(x[m, k]) w[n, k] + bias[n];  q, scale: the 8-bit rows of x (NULL both: nothing is kept)
+ *   backward  x^ = scale q;  dx = (dy w) * act'(x^);  dw = dy^T act(x^);  db = column sums of dy; each written, each may be NULL
+ * Sums in float32; act(x) and act(x^) enter the products rounded to the rows' type.  bias and db of any type, dw of the rows' type or float32.  dx and
+ * q [rows, k] and dw [n, k] without gaps.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and
+ * strides).  Results are the same bits on every run.  The backward wants at least one row; w may be NULL without dx, q and scale where
+ * neither dw nor an activation's dx needs them. */
+int64_t nf_linear_keep_fwd_workspace_bytes(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k, int act);
+int nf_linear_keep_fwd(const void* x, int64_t x_stride, int dtype, const void* w, int64_t w_stride, const void* bias, int bias_dtype, void* y,
+                       int64_t y_stride, int8_t* q, float* scale, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int64_t nf_linear_keep_bwd_workspace_bytes(const void* dy, int64_t dy_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k,
+                                           int need_dx, int need_dw, int need_db);
+int nf_linear_keep_bwd(const void* dy, int64_t dy_stride, int dtype, const int8_t* q, const float* scale, const void* w, int64_t w_stride, void* dx,
+                       void* dw, int dw_dtype, void* db, int db_dtype, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -138,3 +138,60 @@ def test_product_arguments():
         quantize_rows(q)
     with pytest.raises(AssertionError, match="last dimension"):
         quantize_rows(torch.randn(4, 0))
+
+
+def test_keep_entry_points():
+    lib = _lib.load()
+
+    def fwd(x=16, xs=64, dt=BF, w=16, ws=64, bdt=F32, y=16, ys=48, q=16, s=16, rows=4, n=48, k=64, act=0, work=None, size=0):
+        return lib.nf_linear_keep_fwd(x, xs, dt, w, ws, None, bdt, y, ys, q, s, rows, n, k, act, work, size, None)
+
+    refused(fwd(dt=F32), -2, b"float16 or bfloat16")
+    refused(fwd(bdt=5), -1, b"dtype")
+    refused(fwd(act=7), -1, b"activation")
+    for bad in ({"rows": 2**30}, {"rows": -1}, {"n": 0}, {"k": 0}, {"k": 2**29}):
+        refused(fwd(**bad), -1, b"rows")
+    refused(fwd(w=None), -1, b"NULL")
+    refused(fwd(s=None), -1, b"NULL")
+    refused(fwd(xs=63), -1, b"stride")
+    refused(fwd(ws=63), -1, b"stride")
+    refused(fwd(ys=47), -1, b"stride")
+    refused(fwd(act=1), -1, b"workspace")
+    assert fwd(rows=0, x=None) == 0
+    size = lib.nf_linear_keep_fwd_workspace_bytes
+    assert size(16, 64, 16, 64, 4, 48, 64, 0) == 0
+    assert size(16, 64, 16, 64, 4, 48, 64, 1) >= 4 * 64 * 2
+    assert size(18, 64, 16, 64, 4, 48, 64, 0) >= 4 * 64 * 2 and size(16, 64, 18, 64, 4, 48, 64, 0) >= 48 * 64 * 2
+
+    def bwd(dy=16, ds=48, dt=BF, q=16, s=16, w=16, ws=64, dx=16, dw=16, wdt=BF, db=16, bdt=F32, rows=4, n=48, k=64, act=0, work=None, size=0):
+        return lib.nf_linear_keep_bwd(dy, ds, dt, q, s, w, ws, dx, dw, wdt, db, bdt, rows, n, k, act, work, size, None)
+
+    refused(bwd(dt=F32), -2, b"float16 or bfloat16")
+    refused(bwd(wdt=F16), -2, b"weight's gradient")
+    refused(bwd(act=-1), -1, b"activation")
+    refused(bwd(rows=0), -1, b"rows")
+    refused(bwd(dy=None), -1, b"NULL")
+    refused(bwd(q=None), -1, b"NULL")
+    refused(bwd(q=None, dw=None, act=2), -1, b"NULL")
+    refused(bwd(w=None), -1, b"NULL")
+    refused(bwd(ds=47), -1, b"stride")
+    refused(bwd(ws=1), -1, b"stride")
+    need = lib.nf_linear_keep_bwd_workspace_bytes(16, 48, 16, 64, 4, 48, 64, 1, 1, 1)
+    assert need >= 4 * 64 * 2 + 48 * 4
+    refused(bwd(work=16, size=need - 1), -1, b"workspace")
+    refused(bwd(work=8, size=need), -1, b"workspace")
+    assert bwd(dx=None, dw=None, db=None) == 0
+
+
+def test_keep_arguments():
+    from triton_helpers_amd.layers.checkpointed_linear import checkpointed_linear
+
+    x, w, b = torch.randn(4, 64).bfloat16(), torch.randn(48, 64).bfloat16(), torch.randn(48)
+    with pytest.raises(AssertionError, match="GPU"):
+        checkpointed_linear(x, w, b)
+    for bad, word in (((x, w[:, :63], b), "w must be"), ((x, w, b[:3]), "b must be"), ((x, w, b, "tanh"), "activation"), ((x[:, :0], w[:, :0], b), "last dimension")):
+        with pytest.raises(AssertionError, match=word):
+            checkpointed_linear(*bad)
+    for bad in ((x.float(), w.float(), b), (x, w.half(), b), (x, w, b.double())):
+        with pytest.raises(NotImplementedError):
+            checkpointed_linear(*bad)

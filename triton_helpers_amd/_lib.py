@@ -63,6 +63,10 @@ EXPORTS = (
     "nf_quantize_rows",
     "nf_int8_linear",
     "nf_int8_linear_workspace_bytes",
+    "nf_linear_keep_fwd",
+    "nf_linear_keep_fwd_workspace_bytes",
+    "nf_linear_keep_bwd",
+    "nf_linear_keep_bwd_workspace_bytes",
 )
 
 
@@ -161,6 +165,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.nf_int8_linear.argtypes = [P, I64, P, P, I64, P, P, I, P, I64, I, I64, I64, I64, I, P, I64, P]
     lib.nf_int8_linear_workspace_bytes.restype = I64
     lib.nf_int8_linear_workspace_bytes.argtypes = [P, I64, P, I64, I64, I64, I64]
+    lib.nf_linear_keep_fwd.restype = c_int
+    lib.nf_linear_keep_fwd.argtypes = [P, I64, I, P, I64, P, I, P, I64, P, P, I64, I64, I64, I, P, I64, P]
+    lib.nf_linear_keep_fwd_workspace_bytes.restype = I64
+    lib.nf_linear_keep_fwd_workspace_bytes.argtypes = [P, I64, P, I64, I64, I64, I64, I]
+    lib.nf_linear_keep_bwd.restype = c_int
+    lib.nf_linear_keep_bwd.argtypes = [P, I64, I, P, P, P, I64, P, P, I, P, I, I64, I64, I64, I, P, I64, P]
+    lib.nf_linear_keep_bwd_workspace_bytes.restype = I64
+    lib.nf_linear_keep_bwd_workspace_bytes.argtypes = [P, I64, P, I64, I64, I64, I64, I, I, I]
 
 
 def load() -> ctypes.CDLL:

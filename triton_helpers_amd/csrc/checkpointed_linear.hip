@@ -1,0 +1,341 @@
+// A linear layer behind an activation that keeps its input as 8-bit rows for the backward:
+//
+//   forward   y = act(x) W^T + b;                kept: q, s with x^ = s q (quantize_rows.hip), half of what a 16-bit x takes
+//   backward  dx = (dy W) * act'(x^);  dW = dy^T act(x^);  db = sum over rows of dy
+//
+// Three products of 2 M N K operations on the 16-bit matrix instructions (gemm_tile.h).  The forward's lie along the summed dimension; dx takes W,
+// and dW both dy and act(x^), crosswise, as they are in memory.  The gate of dx is applied to the sums in registers.  act(x) and act(x^) are
+// written out in 16 bits by streams of their own (a product reads its operand once for each 256 channels of the result).
+#include "gemm_tile.h"
+
+namespace nf {
+
+enum { OUT_BIAS, OUT_GATE, OUT_PLAIN };
+
+struct Out {
+  void* y;
+  int64_t ldy;
+  const void* bias;
+  int bias_dt, act;
+  const int8_t* q;  // the gate's rows, without gaps
+  const float* s;
+  int m, n, y_dt;
+};
+
+// v * act'(x^); a closed gate lets nothing through, not even an infinity
+template <int ACT>
+__device__ __forceinline__ float gated(float v, float x) {
+  if constexpr (ACT == NF_ACT_NONE) return v;
+  else if constexpr (ACT == NF_ACT_RELU || ACT == NF_ACT_RELU2) return x <= 0.0f ? 0.0f : v * act_slope<ACT>(x);
+  else return v * act_slope<ACT>(x);
+}
+
+template <int MODE, int ACT, typename YT>
+__device__ __forceinline__ void put4(const Out& e, int m, int n, f32x4_t v) {
+  const int left = e.n - n;
+  if constexpr (MODE == OUT_BIAS) {
+    if (e.bias != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += load_as_f32(e.bias, i < left ? n + i : n, e.bias_dt);
+    }
+  }
+  if constexpr (MODE == OUT_GATE && ACT != NF_ACT_NONE) {
+    const int8_t* q = e.q + (int64_t)m * e.n + n;
+    int8_t c[4];
+    if (left >= 4) __builtin_memcpy(c, q, 4);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = q[i < left ? i : 0];
+    const float s = e.s[m];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = gated<ACT>(v[i], s * (float)c[i]);
+  }
+  auto* o = (typename YT::storage*)e.y + (int64_t)m * e.ldy + n;
+  if constexpr (std::is_same<YT, F32>::value) {
+    if (left >= 4) __builtin_memcpy(o, &v, 16);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = v[i];
+  } else {
+    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
+    if (left >= 4) __builtin_memcpy(o, w, 8);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+  }
+}
+// body(activation, type of y) under branches that are the same for every thread
+template <int MODE, typename T, typename Body>
+__device__ __forceinline__ void with_out(const Out& e, Body&& body) {
+  if constexpr (MODE == OUT_GATE) with_act(e.act, [&](auto act_c) { body(act_c, T{}); });
+  else if constexpr (MODE == OUT_BIAS) body(Int<NF_ACT_NONE>{}, T{});
+  else if (e.y_dt == NF_F32) body(Int<NF_ACT_NONE>{}, F32{});
+  else body(Int<NF_ACT_NONE>{}, T{});
+}
+
+template <typename T, typename G, int BM, int BN, int WM, int WN, int MODE>
+__global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, float* slots) {
+  __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
+  f32x4_t acc[G::FM][G::FN] = {};
+  const Tile t = tile_of(g, blockIdx.x);
+  G::run(g, t, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = t.m * BM + wave / WN * (BM / WM) + (lane & 15), n0 = t.n * BN + wave % WN * (BN / WN) + (lane >> 4) * 4;
+  if (slots != nullptr) {  // [split][m][n rounded up to 4]
+    const int64_t ld = (g.n + 3) / 4 * 4;
+    float* o = slots + (int64_t)t.split * g.m * ld;
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) {
+        const int m = m0 + 16 * i, n = n0 + 16 * j;
+        if (m < g.m && n < g.n) *(f32x4_t*)(o + (int64_t)m * ld + n) = acc[i][j];
+      }
+    return;
+  }
+  with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i) {
+      const int m = m0 + 16 * i;
+      if (m >= g.m) continue;
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) {
+        const int n = n0 + 16 * j;
+        if (n < g.n) put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, acc[i][j]);
+      }
+    }
+  });
+}
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits, Out e) {
+  const int64_t quads = (e.n + 3) / 4, ld = quads * 4, each = (int64_t)e.m * ld;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= e.m * quads) return;
+  const int m = (int)(at / quads), n = (int)(at % quads) * 4;
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) v += *(const f32x4_t*)(slots + k * each + (int64_t)m * ld + n);
+  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v); });
+}
+
+// act(s q) in 16 bits, rows filled up with zeros to whole 16-byte pieces; a stream, eight values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void expand_k(const int8_t* q, const float* s, int width, int act, uint16_t* h, int64_t rows) {
+  const int pieces = (width + 7) / 8;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const int64_t row = at / pieces;
+  const int c = (int)(at - row * pieces) * 8, n = width - c;
+  const int8_t* p = q + row * width + c;
+  int8_t raw[8];
+  if (n >= 8) __builtin_memcpy(raw, p, 8);
+  else
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (int8_t)0;
+  const float scale = s[row];
+  with_act(act, [&](auto act_c) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? act_value<decltype(act_c)::value>(scale * (float)raw[i]) : 0.0f;
+    store8<T>(h + at * 8, 8, v);
+  });
+}
+
+// partial column sums: a workgroup takes 256 columns of rows 8 group + 0..7, and every 8 groups on
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_k(const uint16_t* dy, int64_t ld, int64_t rows, int n, float* slots) {
+  __shared__ float part[8][256];
+  const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8, r = threadIdx.x >> 5;
+  float s[8] = {};
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t row = blockIdx.y * 8 + r; row < rows; row += gridDim.y * 8) {
+      float v[8];
+      load8<T>(dy + row * ld + c, n - c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[r][(threadIdx.x & 31) * 8 + i] = s[i];
+  __syncthreads();
+  const int column = blockIdx.x * 256 + threadIdx.x;
+  if (column >= n) return;
+  float v = part[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v += part[i][threadIdx.x];
+  slots[(int64_t)blockIdx.y * n + column] = v;
+}
+
+template <typename T, int MODE, bool AX, bool BX>
+int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream_t s) {
+  g.splits = p.splits;
+  g.split_steps = p.split_steps;
+  const auto go = [&](auto b_c, auto wn_c) {
+    constexpr int B = decltype(b_c)::value, WN = decltype(wn_c)::value;
+    typedef Gemm<T, B, B, 2, WN, 4, AX, BX> G;
+    g.tiles_m = (g.m + B - 1) / B;
+    g.tiles_n = (g.n + B - 1) / B;
+    hipLaunchKernelGGL((keep_tile_k<T, G, B, B, 2, WN, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
+                       p.splits > 1 ? slots : nullptr);
+  };
+  if (p.bm == 256) go(Int<256>{}, Int<4>{});
+  else go(Int<128>{}, Int<2>{});
+  const int rc = check_launch("checkpointed_linear");
+  if (rc != 0 || p.splits == 1) return rc;
+  hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
+  return check_launch("checkpointed_linear_sum");
+}
+
+inline bool sizes_ok(int64_t rows, int64_t n, int64_t k) {
+  return rows > 0 && rows < (1ll << 30) && n >= 1 && n < (1ll << 29) && k >= 1 && k < (1ll << 29);
+}
+
+struct KeepFwd {
+  int64_t ldh, h_bytes, w_bytes;
+  TilePlan tile;
+  int64_t total() const { return h_bytes + w_bytes + tile.slot_bytes; }
+};
+KeepFwd keep_fwd(const void* x, int64_t xs, const void* w, int64_t ws, int64_t rows, int64_t n, int64_t k, int act) {
+  KeepFwd p{};
+  p.ldh = round_up(k, 8);
+  if (act != NF_ACT_NONE || !rows_fit(x, xs * 2, k * 2)) p.h_bytes = round_up(rows * p.ldh * 2, 256);
+  if (!rows_fit(w, ws * 2, k * 2)) p.w_bytes = round_up(n * p.ldh * 2, 256);
+  p.tile = tile_plan(rows, n, k * 2);
+  return p;
+}
+
+struct KeepBwd {
+  int64_t ldk, ldn, dy_bytes, w_bytes, h_bytes, sum_bytes;
+  int strips, groups;
+  TilePlan dx, dw;
+  int64_t slots() const { return dx.slot_bytes > dw.slot_bytes ? dx.slot_bytes : dw.slot_bytes; }
+  int64_t total() const { return dy_bytes + w_bytes + h_bytes + sum_bytes + slots(); }
+};
+KeepBwd keep_bwd(const void* dy, int64_t dys, const void* w, int64_t ws, int64_t rows, int64_t n, int64_t k, bool need_dx, bool need_dw, bool need_db) {
+  KeepBwd p{};
+  p.ldk = round_up(k, 8);
+  p.ldn = round_up(n, 8);
+  if ((need_dx || need_dw) && !rows_fit(dy, dys * 2, n * 2)) p.dy_bytes = round_up(rows * p.ldn * 2, 256);
+  if (need_dx) {
+    if (!rows_fit(w, ws * 2, k * 2)) p.w_bytes = round_up(n * p.ldk * 2, 256);
+    p.dx = tile_plan(rows, k, n * 2);
+  }
+  if (need_dw) {
+    p.h_bytes = round_up(rows * p.ldk * 2, 256);
+    p.dw = tile_plan(n, k, rows * 2);
+  }
+  if (need_db) {
+    p.strips = (int)((n + 255) / 256);
+    const int64_t most = 1024 / p.strips + 1, want = (rows + 63) / 64;
+    p.groups = (int)(want < most ? want : most);
+    p.sum_bytes = round_up((int64_t)p.groups * n * 4, 256);
+  }
+  return p;
+}
+
+template <typename T>
+int fwd(const KeepFwd& p, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, int bias_dt, void* y, int64_t ys, int8_t* q, float* scale,
+        int64_t rows, int64_t n, int64_t k, int act, char* at, void* stream) {
+  char *h = at, *packed = at + p.h_bytes;
+  float* slots = (float*)(packed + p.w_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  if (q != nullptr || p.h_bytes > 0)
+    if (const int rc = nf_quantize_rows(x, xs, T::code, q, scale, p.h_bytes > 0 ? h : nullptr, p.ldh, act, rows, k, stream)) return rc;
+  if (p.w_bytes > 0)
+    if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed, n, s)) return rc;
+  const GemmArgs g{p.h_bytes > 0 ? h : (const char*)x, p.w_bytes > 0 ? packed : (const char*)w, (p.h_bytes > 0 ? p.ldh : xs) * 2,
+                   (p.w_bytes > 0 ? p.ldh : ws) * 2, (int)rows, (int)n, (int)k * 2, 0, 0, 0, 0};
+  const Out e{y, ys, bias, bias_dt, NF_ACT_NONE, nullptr, nullptr, (int)rows, (int)n, T::code};
+  return product<T, OUT_BIAS, false, false>(g, p.tile, e, slots, s);
+}
+
+template <typename T>
+int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const float* scale, const void* w, int64_t ws, void* dx, void* dw, int dw_dt,
+        void* db, int db_dt, int64_t rows, int64_t n, int64_t k, int act, char* at, hipStream_t s) {
+  char *packed_dy = at, *packed_w = packed_dy + p.dy_bytes, *h = packed_w + p.w_bytes, *sums = h + p.h_bytes;
+  float* slots = (float*)(sums + p.sum_bytes);
+  if (db != nullptr) {
+    hipLaunchKernelGGL((column_sums_k<T>), dim3(p.strips, p.groups), dim3(256), 0, s, (const uint16_t*)dy, dys, rows, (int)n, (float*)sums);
+    if (const int rc = check_launch("column_sums")) return rc;
+    if (const int rc = sum_slots((const float*)sums, p.groups, n, db, db_dt, s)) return rc;
+  }
+  const char* a = (const char*)dy;
+  int64_t lda = dys * 2;
+  if (p.dy_bytes > 0) {
+    if (const int rc = pack_rows(a, lda, n * 2, packed_dy, rows, s)) return rc;
+    a = packed_dy;
+    lda = p.ldn * 2;
+  }
+  if (dx != nullptr) {
+    if (p.w_bytes > 0)
+      if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed_w, n, s)) return rc;
+    const GemmArgs g{a, p.w_bytes > 0 ? packed_w : (const char*)w, lda, (p.w_bytes > 0 ? p.ldk : ws) * 2, (int)rows, (int)k, (int)n * 2, 0, 0, 0, 0};
+    const Out e{dx, k, nullptr, NF_F32, act, q, scale, (int)rows, (int)k, T::code};
+    if (const int rc = product<T, OUT_GATE, false, true>(g, p.dx, e, slots, s)) return rc;
+  }
+  if (dw != nullptr) {
+    const int64_t pieces = rows * (p.ldk / 8);
+    hipLaunchKernelGGL((expand_k<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, q, scale, (int)k, act, (uint16_t*)h, rows);
+    if (const int rc = check_launch("expand")) return rc;
+    const GemmArgs g{a, h, lda, p.ldk * 2, (int)n, (int)k, (int)rows * 2, 0, 0, 0, 0};
+    const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt};
+    if (const int rc = product<T, OUT_PLAIN, true, true>(g, p.dw, e, slots, s)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace nf
+
+using namespace nf;
+
+extern "C" int64_t nf_linear_keep_fwd_workspace_bytes(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k,
+                                                      int act) {
+  return sizes_ok(rows, n, k) ? keep_fwd(x, x_stride, w, w_stride, rows, n, k, act).total() : 0;
+}
+
+extern "C" int nf_linear_keep_fwd(const void* x, int64_t x_stride, int dtype, const void* w, int64_t w_stride, const void* bias, int bias_dtype, void* y,
+                                  int64_t y_stride, int8_t* q, float* scale, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  NF_REQUIRE(dtype == NF_F16 || dtype == NF_BF16, NF_EUNSUPPORTED, "dtype code %d: float16 or bfloat16 rows", dtype);
+  NF_REQUIRE(dtype_ok(bias_dtype), NF_EINVAL, "unknown dtype code %d", bias_dtype);
+  NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
+  if (rows == 0) return 0;
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows below 2^30, channels 1..2^29-1", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(x && w && y && (q == nullptr) == (scale == nullptr), NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE((rows == 1 || (x_stride >= k && y_stride >= n)) && (n == 1 || w_stride >= k), NF_EINVAL, "row stride below the row's length");
+  const KeepFwd p = keep_fwd(x, x_stride, w, w_stride, rows, n, k, act);
+  NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
+             "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
+  return dtype == NF_F16 ? fwd<F16>(p, x, x_stride, w, w_stride, bias, bias_dtype, y, y_stride, q, scale, rows, n, k, act, (char*)workspace, stream)
+                         : fwd<BF16>(p, x, x_stride, w, w_stride, bias, bias_dtype, y, y_stride, q, scale, rows, n, k, act, (char*)workspace, stream);
+}
+
+extern "C" int64_t nf_linear_keep_bwd_workspace_bytes(const void* dy, int64_t dy_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k,
+                                                      int need_dx, int need_dw, int need_db) {
+  return sizes_ok(rows, n, k) ? keep_bwd(dy, dy_stride, w, w_stride, rows, n, k, need_dx != 0, need_dw != 0, need_db != 0).total() : 0;
+}
+
+extern "C" int nf_linear_keep_bwd(const void* dy, int64_t dy_stride, int dtype, const int8_t* q, const float* scale, const void* w, int64_t w_stride, void* dx,
+                                  void* dw, int dw_dtype, void* db, int db_dtype, int64_t rows, int64_t n, int64_t k, int act, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  NF_REQUIRE(dtype == NF_F16 || dtype == NF_BF16, NF_EUNSUPPORTED, "dtype code %d: float16 or bfloat16 rows", dtype);
+  NF_REQUIRE((dw_dtype == dtype || dw_dtype == NF_F32) && dtype_ok(db_dtype), NF_EUNSUPPORTED, "the weight's gradient is of the rows' type or float32");
+  NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows 1..2^30-1, channels 1..2^29-1", (long long)rows, (long long)n, (long long)k);
+  if (dx == nullptr && dw == nullptr && db == nullptr) return 0;
+  NF_REQUIRE(dy && (db != nullptr || dw != nullptr || dx != nullptr), NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE(dw == nullptr || (q && scale), NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE(dx == nullptr || (w && (act == NF_ACT_NONE || (q && scale))), NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE((rows == 1 || dy_stride >= n) && (n == 1 || dx == nullptr || w_stride >= k), NF_EINVAL, "row stride below the row's length");
+  const KeepBwd p = keep_bwd(dy, dy_stride, w, w_stride, rows, n, k, dx != nullptr, dw != nullptr, db != nullptr);
+  NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
+             "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == NF_F16
+             ? bwd<F16>(p, dy, dy_stride, q, scale, w, w_stride, dx, dw, dw_dtype, db, db_dtype, rows, n, k, act, (char*)workspace, s)
+             : bwd<BF16>(p, dy, dy_stride, q, scale, w, w_stride, dx, dw, dw_dtype, db, db_dtype, rows, n, k, act, (char*)workspace, s);
+}

@@ -317,8 +317,160 @@ PyObject* int8_linear_launch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ linear layer with 8-bit checkpoints
+struct Keep {
+  Tensor x, w, b;  // b: undefined without
+  int act;
+};
+
+bool keep_fits(const Keep& m, bool cast) {
+  if (m.x.dim() < 1 || m.w.dim() != 2 || m.x.size(-1) < 1 || m.w.size(0) < 1 || m.w.size(1) != m.x.size(-1) || m.w.device() != m.x.device()) return false;
+  if (m.b.defined() && (!float_type(m.b) || m.b.dim() != 1 || m.b.size(0) != m.w.size(0) || m.b.device() != m.x.device())) return false;
+  const auto half = [](const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; };
+  return cast ? float_type(m.x) && float_type(m.w) : half(m.x) && m.w.scalar_type() == m.x.scalar_type();
+}
+
+// (y, q, scale); the last two only where they are kept
+variable_list keep_forward(const Keep& m, bool keep) {
+  const c10::DeviceGuard guard(m.x.device());
+  const int64_t k = m.x.size(-1), n = m.w.size(0);
+  const Rows x(m.x, k), w(m.w, k);
+  const Tensor b = contiguous(m.b);
+  c10::SmallVector<int64_t, 5> shape(m.x.sizes().begin(), m.x.sizes().end());
+  shape.back() = n;
+  const Tensor y = at::empty(shape, m.x.options());
+  Tensor q, scale;
+  if (keep) {
+    q = at::empty(m.x.sizes(), m.x.options().dtype(at::kChar));
+    scale = at::empty({x.n}, m.x.options().dtype(at::kFloat));
+  }
+  if (x.n > 0) {
+    const int64_t bytes = nf_linear_keep_fwd_workspace_bytes(x.p, x.stride, w.p, w.stride, x.n, n, k, m.act);
+    const Tensor ws = scratch(bytes, m.x);
+    check(nf_linear_keep_fwd(x.p, x.stride, code_of(m.x.scalar_type()), w.p, w.stride, ptr(b), b.defined() ? code_of(b.scalar_type()) : NF_F32, y.data_ptr(),
+                             n, (int8_t*)ptr(q), (float*)ptr(scale), x.n, n, k, m.act, ptr(ws), bytes, stream_of(m.x)),
+          "nf_linear_keep_fwd");
+  }
+  return {y, q, scale};
+}
+
+// (dx, dw, db); dw in float32 where `float_dw`, db of type `bt`
+variable_list keep_backward(const Tensor& q, const Tensor& scale, const Tensor& weight, int act, Tensor dy, bool need_dx, bool need_dw, bool need_db,
+                            bool float_dw, at::ScalarType bt) {
+  const c10::DeviceGuard guard(weight.device());
+  const int64_t n = weight.size(0), k = weight.size(1);
+  if (dy.scalar_type() != weight.scalar_type()) dy = dy.to(weight.scalar_type());
+  const Rows g(dy, n), w(weight, k);
+  Tensor dx, dw, db;
+  c10::SmallVector<int64_t, 5> shape(dy.sizes().begin(), dy.sizes().end());
+  shape.back() = k;
+  if (need_dx) dx = at::empty(shape, weight.options());
+  const auto made = [&](at::IntArrayRef sizes, at::ScalarType t) {
+    return g.n > 0 ? at::empty(sizes, weight.options().dtype(t)) : at::zeros(sizes, weight.options().dtype(t));
+  };
+  if (need_dw) dw = made({n, k}, float_dw ? at::kFloat : weight.scalar_type());
+  if (need_db) db = made({n}, bt);
+  if (g.n > 0) {
+    const int64_t bytes = nf_linear_keep_bwd_workspace_bytes(g.p, g.stride, w.p, w.stride, g.n, n, k, need_dx, need_dw, need_db);
+    const Tensor ws = scratch(bytes, weight);
+    check(nf_linear_keep_bwd(g.p, g.stride, code_of(weight.scalar_type()), (const int8_t*)ptr(q), (const float*)ptr(scale), w.p, w.stride, ptr(dx), ptr(dw),
+                             dw.defined() ? code_of(dw.scalar_type()) : NF_F32, ptr(db), code_of(bt), g.n, n, k, act, ptr(ws), bytes, stream_of(weight)),
+          "nf_linear_keep_bwd");
+  }
+  return {dx, dw, db};
+}
+
+struct LinearKeep : torch::autograd::Function<LinearKeep> {
+  // cast: the type that autocast asks for, or the tensors' own
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, std::optional<Tensor> b, int64_t act, int64_t cast) {
+    const auto type = (at::ScalarType)cast;
+    const bool keep = w.requires_grad() || act != NF_ACT_NONE;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Keep m{x.to(type), w.to(type), b.value_or(Tensor()), (int)act};
+    const variable_list r = keep_forward(m, keep);
+    ctx->save_for_backward({r[1], r[2], m.w});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["float_dw"] = w.scalar_type() == at::kFloat;
+    ctx->saved_data["bias"] = b ? (int64_t)b->scalar_type() : (int64_t)-1;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t bias = ctx->saved_data["bias"].toInt();
+    variable_list g = keep_backward(s[0], s[1], s[2], (int)ctx->saved_data["act"].toInt(), grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                    bias >= 0 && ctx->needs_input_grad(2), ctx->saved_data["float_dw"].toBool(),
+                                    bias >= 0 ? (at::ScalarType)bias : at::kFloat);
+    g.resize(5);
+    return g;
+  }
+};
+
+// checkpointed_linear(x, w, b, activation)
+PyObject* checkpointed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  Keep m;
+  std::optional<Tensor> b;
+  m.act = activation(a[3], true);
+  if (modes_active() || m.act < 0 || !plain(a[0], &m.x) || !plain(a[1], &m.w) || !plain_or_none(a[2], &b)) Py_RETURN_NONE;
+  m.b = b.value_or(Tensor());
+  const bool cast = autocast();
+  if (!keep_fits(m, cast)) Py_RETURN_NONE;
+  const at::ScalarType type = cast ? at::autocast::get_autocast_dtype(at::kCUDA) : m.x.scalar_type();
+  if (type != at::kHalf && type != at::kBFloat16) Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release release;
+    if (needs_grad(m.x) || needs_grad(m.w) || needs_grad(m.b)) {
+      y = LinearKeep::apply(m.x, m.w, b, (int64_t)m.act, (int64_t)type);
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      y = keep_forward(Keep{m.x.to(type), m.w.to(type), m.b, m.act}, false)[0];
+    }
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// checkpointed_linear_launch_forward(x, w, b, activation code) on checked arguments: (y, q, scale)
+PyObject* checkpointed_linear_launch_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(4);
+  int64_t act;
+  TORCH_CHECK(as_int(a[3], &act), "activation code expected");
+  const Keep m{tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]), (int)act};
+  variable_list r;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    r = keep_forward(m, true);
+  }
+  return wrap_list(r);
+  END_HANDLE_TH_ERRORS
+}
+
+// checkpointed_linear_launch_backward(q, scale, w, activation code, dy, need_dx, need_dw, need_db, float_dw, code of db's type): (dx, dw, db)
+PyObject* checkpointed_linear_launch_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  NARGS(10);
+  int64_t act, bt;
+  TORCH_CHECK(as_int(a[3], &act) && as_int(a[9], &bt), "codes expected");
+  const Tensor q = tensor_arg(a[0]), scale = tensor_arg(a[1]), w = tensor_arg(a[2]), dy = tensor_arg(a[4]);
+  const bool dx = a[5] == Py_True, dw = a[6] == Py_True, db = a[7] == Py_True, wide = a[8] == Py_True;
+  variable_list r;
+  {
+    pybind11::gil_scoped_release release;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    r = keep_backward(q, scale, w, (int)act, dy, dx, dw, db, wide, bt == NF_F32 ? at::kFloat : bt == NF_F16 ? at::kHalf : at::kBFloat16);
+  }
+  return wrap_list(r);
+  END_HANDLE_TH_ERRORS
+}
+
 }  // namespace
 
 PyMethodDef wide_methods[] = {ENTRY(rms_norm), ENTRY(rms_norm_int8), ENTRY(rms_norm_launch_forward), ENTRY(rms_norm_launch_backward),
                               ENTRY(quantize_rows), ENTRY(quantize_rows_launch), ENTRY(int8_linear), ENTRY(int8_linear_launch),
+                              ENTRY(checkpointed_linear), ENTRY(checkpointed_linear_launch_forward), ENTRY(checkpointed_linear_launch_backward),
                               {nullptr, nullptr, 0, nullptr}};

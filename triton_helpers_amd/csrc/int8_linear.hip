@@ -208,36 +208,28 @@ __global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld,
   *(i32x4_t*)(to + row * pieces * 16 + k) = load16(from + row * ld, k, bytes);
 }
 
-struct Plan {
-  bool few;
-  int bm, splits, split_steps;
-  bool pack_q, pack_w;
-  int64_t q_bytes, w_bytes, slot_bytes;
-  int64_t total() const { return q_bytes + w_bytes + slot_bytes; }
-};
-
-inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
-inline bool rows_fit(const void* p, int64_t ld, int64_t k) { return k % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
+int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s) {
+  const int64_t pieces = (bytes + 15) / 16;
+  hipLaunchKernelGGL(pack_rows_k, dim3((unsigned)((rows * pieces + 255) / 256)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
+  return check_launch("pack_rows");
+}
 
 constexpr int FEW_ROWS = 64;
+
+struct Plan {
+  bool few;
+  TilePlan tile;
+  int64_t q_bytes, w_bytes;  // of packed copies
+  int64_t total() const { return q_bytes + w_bytes + tile.slot_bytes; }
+};
 
 Plan plan(const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t m, int64_t n, int64_t k) {
   Plan p{};
   p.few = m <= FEW_ROWS;
   if (p.few) return p;
-  p.pack_q = !rows_fit(q, ldq, k);
-  p.pack_w = !rows_fit(w, ldw, k);
-  if (p.pack_q) p.q_bytes = round_up(m * round_up(k, 16), 256);
-  if (p.pack_w) p.w_bytes = round_up(n * round_up(k, 16), 256);
-  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-  p.bm = big >= 192 ? 256 : 128;
-  const int64_t tiles = p.bm == 256 ? big : small, steps = (k + STEP - 1) / STEP;
-  int64_t splits = p.bm == 256 ? 1 : 512 / tiles;
-  if (splits > steps / 8) splits = steps / 8;
-  if (splits < 1) splits = 1;
-  p.split_steps = (int)((steps + splits - 1) / splits);
-  p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
-  if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 4) * 4, 256);
+  if (!rows_fit(q, ldq, k)) p.q_bytes = round_up(m * round_up(k, 16), 256);
+  if (!rows_fit(w, ldw, k)) p.w_bytes = round_up(n * round_up(k, 16), 256);
+  p.tile = tile_plan(m, n, k);
   return p;
 }
 
@@ -290,25 +282,20 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   char* ws = (char*)workspace;
   const char *a = (const char*)q, *b = (const char*)w;
   int64_t lda = q_stride, ldb = w_stride;
-  const auto pack = [&](const char* from, int64_t ld, int64_t count, char* to) {
-    const int64_t pieces = (k + 15) / 16;
-    hipLaunchKernelGGL(pack_rows_k, dim3((unsigned)((count * pieces + 255) / 256)), dim3(256), 0, s, from, ld, (int)k, to, count);
-    return check_launch("pack_rows");
-  };
-  if (p.pack_q) {
-    if (const int rc = pack(a, lda, rows, ws)) return rc;
+  if (p.q_bytes > 0) {
+    if (const int rc = pack_rows(a, lda, k, ws, rows, s)) return rc;
     a = ws;
     lda = round_up(k, 16);
   }
-  if (p.pack_w) {
-    if (const int rc = pack(b, ldb, n, ws + p.q_bytes)) return rc;
+  if (p.w_bytes > 0) {
+    if (const int rc = pack_rows(b, ldb, k, ws + p.q_bytes, n, s)) return rc;
     b = ws + p.q_bytes;
     ldb = round_up(k, 16);
   }
-  const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)round_up(k, 16), 0, 0, p.splits, p.split_steps};
-  int* slots = p.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
-  const int rc = p.bm == 256 ? tile_launch<256, 256, 2, 4, 4>(g, e, slots, s) : tile_launch<128, 128, 2, 2, 4>(g, e, slots, s);
+  const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)k, 0, 0, p.tile.splits, p.tile.split_steps};
+  int* slots = p.tile.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
+  const int rc = p.tile.bm == 256 ? tile_launch<256, 256, 2, 4, 4>(g, e, slots, s) : tile_launch<128, 128, 2, 2, 4>(g, e, slots, s);
   if (rc != 0 || slots == nullptr) return rc;
-  hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
+  hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.tile.splits, e);
   return check_launch("int8_sum");
 }

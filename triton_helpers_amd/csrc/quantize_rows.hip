@@ -8,7 +8,7 @@ namespace nf {
 
 struct Quantize {
   const void* x;
-  int8_t* q;
+  int8_t* q;  // NULL: h alone
   float* scale;
   void* h;  // NULL, or rows of x's type with `hs` values between them; values behind the row's end become zeros
   int64_t xs, hs, rows;
@@ -48,6 +48,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_k(Quantize a) {
   if constexpr (KEEP) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) put_act<XT, ACT>(a, row, (j * T + t) * 8, v[j]);
+    if (a.q == nullptr) return;
   }
   const EightBit e = eight_bit(row_max<T>(top, tops));
   if (t == 0) a.scale[row] = e.scale;
@@ -76,6 +77,7 @@ __global__ __launch_bounds__(1024) void quantize_wide_k(Quantize a) {
     }
     if constexpr (KEEP) put_act<XT, ACT>(a, row, c, v);
   }
+  if (KEEP && a.q == nullptr) return;
   const EightBit e = eight_bit(row_max<1024>(top, tops));
   if (threadIdx.x == 0) a.scale[row] = e.scale;
   for (int c = threadIdx.x * 8; c < a.width; c += 8192) {
@@ -127,7 +129,7 @@ extern "C" int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, in
   NF_REQUIRE(h == nullptr || h_stride == width || h_stride == (width + 7) / 8 * 8, NF_EINVAL, "h_stride=%lld: the width, or the next multiple of 8",
              (long long)h_stride);
   if (rows == 0) return 0;
-  NF_REQUIRE(x && q && scale, NF_EINVAL, "NULL pointer argument");
+  NF_REQUIRE(x && (q ? scale != nullptr : h != nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE(rows == 1 || x_stride >= width, NF_EINVAL, "row stride below the width");
   const Quantize a{x, q, scale, h, x_stride, h_stride, rows, (int)width};
   hipStream_t s = (hipStream_t)stream;

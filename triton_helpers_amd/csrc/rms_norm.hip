@@ -275,8 +275,8 @@ __global__ __launch_bounds__(1024) void rms_bwd_wide_k(NormBwd a) {
   }
 }
 
-// dw: the groups' partial sums, in a fixed order (the same bits on every run)
-__global__ __launch_bounds__(1024) void rms_dw_k(const float* slots, int64_t groups, int width, void* dw, int wt) {
+// column sums of the groups' partial sums, in a fixed order (the same bits on every run)
+__global__ __launch_bounds__(1024) void sum_slots_k(const float* slots, int64_t groups, int width, void* out, int dt) {
   __shared__ float part[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
   float s = 0.0f;
@@ -289,8 +289,13 @@ __global__ __launch_bounds__(1024) void rms_dw_k(const float* slots, int64_t gro
   if (g == 0 && c < width) {
 #pragma unroll
     for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
-    store_any(dw, c, wt, s);
+    store_any(out, c, dt, s);
   }
+}
+
+int sum_slots(const float* slots, int64_t groups, int64_t width, void* out, int dt, hipStream_t s) {
+  hipLaunchKernelGGL(sum_slots_k, dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, s, slots, groups, (int)width, out, dt);
+  return check_launch("sum_slots");
 }
 
 constexpr int NORM_ONE_PASS = 32768;  // the widest row that a workgroup's registers hold
@@ -401,7 +406,5 @@ extern "C" int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, c
   else if (x_dtype == NF_F16) rc = h_dtype == NF_F32 ? bwd_launch<F16, F32>(a, groups, s) : bwd_launch<F16, F16>(a, groups, s);
   else rc = h_dtype == NF_F32 ? bwd_launch<BF16, F32>(a, groups, s) : bwd_launch<BF16, BF16>(a, groups, s);
   if (rc != 0 || dw == nullptr) return rc;
-  hipLaunchKernelGGL(rms_dw_k, dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, s, (const float*)workspace, slot_rows(rows, (int)width), (int)width, dw,
-                     weight_dtype);
-  return check_launch("rms_norm_dw");
+  return sum_slots((const float*)workspace, slot_rows(rows, (int)width), width, dw, weight_dtype, s);
 }

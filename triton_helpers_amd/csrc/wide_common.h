@@ -151,4 +151,7 @@ __device__ __forceinline__ float act_slope(float z) {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
+// out[c] = sum over `groups` rows of `slots` (rms_norm.hip)
+int sum_slots(const float* slots, int64_t groups, int64_t width, void* out, int dt, hipStream_t s);
+
 }  // namespace nf
