@@ -195,3 +195,22 @@ def test_keep_arguments():
     for bad in ((x.float(), w.float(), b), (x, w.half(), b), (x, w, b.double())):
         with pytest.raises(NotImplementedError):
             checkpointed_linear(*bad)
+
+
+def test_alias_package_and_names():
+    """The wide layers resolve through ``triton_helpers.layers`` as the others do."""
+    import triton_helpers.layers.checkpointed_linear as c
+    import triton_helpers.layers.int8_linear as i
+    import triton_helpers.layers.rms_norm as r
+    import triton_helpers.layers.wide_mlp as w
+
+    from triton_helpers_amd.layers import checkpointed_linear, int8_linear, rms_norm, wide_mlp
+
+    for alias, own in ((c, checkpointed_linear), (i, int8_linear), (r, rms_norm), (w, wide_mlp)):
+        assert sorted(alias.__all__) == sorted(own.__all__)
+        assert all(getattr(alias, n) is getattr(own, n) for n in own.__all__)
+    m = w.WideMLP(96, 384)
+    assert {k: tuple(v.shape) for k, v in m.state_dict().items()} == {
+        "norm.weight": (96,), "up.weight": (384, 96), "up.bias": (384,), "down.weight": (96, 384), "down.bias": (96,)}
+    with pytest.raises(AssertionError, match="GPU"):
+        m.to_int8()
