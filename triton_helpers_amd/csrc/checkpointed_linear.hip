@@ -30,42 +30,31 @@ __device__ __forceinline__ float gated(float v, float x) {
   else return v * act_slope<ACT>(x);
 }
 
-template <int MODE, int ACT, typename YT>
-__device__ __forceinline__ void put4(const Out& e, int m, int n, f32x4_t v) {
+// four values of the gate's rows; a NaN scale stays one
+__device__ __forceinline__ int gate4(const Out& e, int m, int n) {
+  const int8_t* q = e.q + (int64_t)m * e.n + n;
+  int8_t c[4];
   const int left = e.n - n;
-  if constexpr (MODE == OUT_BIAS) {
-    if (e.bias != nullptr) {
+  if (left >= 4) __builtin_memcpy(c, q, 4);
+  else
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += load_as_f32(e.bias, i < left ? n + i : n, e.bias_dt);
-    }
-  }
-  if constexpr (MODE == OUT_GATE && ACT != NF_ACT_NONE) {
-    const int8_t* q = e.q + (int64_t)m * e.n + n;
-    int8_t c[4];
-    if (left >= 4) __builtin_memcpy(c, q, 4);
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = q[i < left ? i : 0];
-    const float s = e.s[m];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = gated<ACT>(v[i], s * (float)c[i]);
-  }
-  auto* o = (typename YT::storage*)e.y + (int64_t)m * e.ldy + n;
-  if constexpr (std::is_same<YT, F32>::value) {
-    if (left >= 4) __builtin_memcpy(o, &v, 16);
-    else
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = v[i];
-  } else {
-    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
-    if (left >= 4) __builtin_memcpy(o, w, 8);
-    else
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-  }
+    for (int i = 0; i < 4; ++i) c[i] = q[i < left ? i : 0];
+  return __builtin_bit_cast(int, c);
 }
+
+// four columns of a row: b the columns' biases; q, s the gate's values and scale
+template <int MODE, int ACT, typename YT>
+__device__ __forceinline__ void put4(const Out& e, int m, int n, f32x4_t v, const float (&b)[4], int q, float s) {
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (MODE == OUT_BIAS) r[i] = v[i] + b[i];
+    else if constexpr (MODE == OUT_GATE) r[i] = gated<ACT>(v[i], s * (float)(q << (24 - 8 * i) >> 24));
+    else r[i] = v[i];
+  }
+  store4<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, r);
+}
+
 // body(activation, type of y) under branches that are the same for every thread
 template <int MODE, typename T, typename Body>
 __device__ __forceinline__ void with_out(const Out& e, Body&& body) {
@@ -95,6 +84,22 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
       }
     return;
   }
+  // what the results go together with is asked for at once
+  float b[G::FN][4] = {}, s[G::FM] = {};
+  int q[G::FM][G::FN] = {};
+  if (MODE == OUT_BIAS && e.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < G::FN; ++j) load4(e.bias, e.bias_dt, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1, g.n, b[j]);
+  }
+  if (MODE == OUT_GATE && e.act != NF_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i) {
+      const int m = m0 + 16 * i < g.m ? m0 + 16 * i : g.m - 1;
+      s[i] = e.s[m];
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) q[i][j] = gate4(e, m, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1);
+    }
+  }
   with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
 #pragma unroll
     for (int i = 0; i < G::FM; ++i) {
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
 #pragma unroll
       for (int j = 0; j < G::FN; ++j) {
         const int n = n0 + 16 * j;
-        if (n < g.n) put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, acc[i][j]);
+        if (n < g.n) put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, acc[i][j], b[j], q[i][j], s[i]);
       }
     }
   });
@@ -118,7 +123,14 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
   f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int k = 0; k < splits; ++k) v += *(const f32x4_t*)(slots + k * each + (int64_t)m * ld + n);
-  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v); });
+  float b[4] = {}, s = 0.0f;
+  int q = 0;
+  if (MODE == OUT_BIAS && e.bias != nullptr) load4(e.bias, e.bias_dt, n, e.n, b);
+  if (MODE == OUT_GATE && e.act != NF_ACT_NONE) {
+    q = gate4(e, m, n);
+    s = e.s[m];
+  }
+  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b, q, s); });
 }
 
 // act(s q) in 16 bits, rows filled up with zeros to whole 16-byte pieces; a stream, eight values a thread
@@ -174,16 +186,18 @@ template <typename T, int MODE, bool AX, bool BX>
 int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream_t s) {
   g.splits = p.splits;
   g.split_steps = p.split_steps;
-  const auto go = [&](auto b_c, auto wn_c) {
-    constexpr int B = decltype(b_c)::value, WN = decltype(wn_c)::value;
-    typedef Gemm<T, B, B, 2, WN, 4, AX, BX> G;
+  const auto go = [&](auto b_c, auto wm_c, auto wn_c) {
+    constexpr int B = decltype(b_c)::value, WM = decltype(wm_c)::value, WN = decltype(wn_c)::value;
+    typedef Gemm<T, B, B, WM, WN, AX, BX> G;
     g.tiles_m = (g.m + B - 1) / B;
     g.tiles_n = (g.n + B - 1) / B;
-    hipLaunchKernelGGL((keep_tile_k<T, G, B, B, 2, WN, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
+    hipLaunchKernelGGL((keep_tile_k<T, G, B, B, WM, WN, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
                        p.splits > 1 ? slots : nullptr);
   };
-  if (p.bm == 256) go(Int<256>{}, Int<4>{});
-  else go(Int<128>{}, Int<2>{});
+  // (waves of 64 x 128 are 2 % quicker than 128 x 64 where both operands lie along the sum, 2 to 5 % slower where one is crosswise)
+  if (p.bm == 128) go(Int<128>{}, Int<2>{}, Int<2>{});
+  else if constexpr (AX || BX) go(Int<256>{}, Int<2>{}, Int<4>{});
+  else go(Int<256>{}, Int<4>{}, Int<2>{});
   const int rc = check_launch("checkpointed_linear");
   if (rc != 0 || p.splits == 1) return rc;
   hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);

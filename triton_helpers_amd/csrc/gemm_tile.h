@@ -2,10 +2,13 @@
 // (16x16x32, float32 sums).  Both take 16 bytes a lane and 64 bytes of a row and step, so the code sees bytes.  Operands of 16 bits may also lie
 // across the summed dimension, A as [k][m] or B as [k][n] ("crosswise"): LDS's transposing read hands them to the instruction.
 //
-// A workgroup owns BM x BN of C.  Steps of 64 bytes of every row of its operands go straight from memory to
-// LDS (no registers in between) into a ring of S slots; S - 1 are in flight or waiting.  A wave keeps the operands of the step that it multiplies
-// in registers and reads the next step's between the matrix instructions.  16-byte pieces of a row are placed by an exclusive-or with
-// the row's number, which spreads the sixteen rows that a read touches over all banks.
+// A workgroup owns BM x BN of C.  Steps of 128 bytes of every row of its operands (whole cache lines: with 64 bytes the L2 hands out twice
+// the bytes, 0.40 us instead of 0.27 for 32 KB on all compute units) go straight from memory to LDS, no registers in between, into a ring of five
+// slots, each one operand's step: A, B, A, B, A.  A step is multiplied in two halves; a wave keeps the operands of the half that it multiplies in
+// registers and reads the next half's between the matrix instructions.  There is one meeting of the waves in a step, behind its first half: then
+// all of the step is in registers, its two slots are free, and the next step has to be there.
+//
+// bf16 16384 x 4096 x 4096 on tiles of 256 x 256: RATE_NT
 //
 // Rows start on 16-byte boundaries and hold whole 16-byte pieces (along the summed dimension: with zeros behind the last value).  Rows of C beyond
 // the operand repeat its last one, columns of a crosswise operand beyond it are whatever the buffer holds: neither is stored.  What lies
@@ -44,7 +47,7 @@ struct Mma<BF16> {
   }
 };
 
-constexpr int STEP = 64;  // bytes of a row in one step
+constexpr int STEP = 128, HALF = 64;  // bytes of a row in one step, and in one matrix instruction
 
 struct GemmArgs {
   const char *a, *b;
@@ -89,18 +92,19 @@ __device__ __forceinline__ void load_to_lds(i32x4_t buffer, int offset, uint32_t
 
 // One operand of a workgroup: R rows of C's side, and the loads that bring a step of it to LDS.
 //
-// Along the summed dimension a step is R rows of 64 bytes; piece p of row r lies at place p ^ (r / 4).  Crosswise it is 32 rows of 2 R bytes; the
-// 32-byte segments, sixteen values that one transposing read takes from each of sixteen rows, are spread over the banks by
-// an exclusive-or with the row's bits 0, 1 and 3.
+// Along the summed dimension a step is R rows of 128 bytes; piece p (16 bytes) of row r lies at place p ^ (r / 2 % 8).  Crosswise it is 64 rows of 2 R bytes;
+// the 32-byte segments, sixteen values that one transposing read takes from each of sixteen rows, are spread over the banks by
+// an exclusive-or with the row's bits 0, 1 and 3.  No read meets a bank twice that way (a wave's 16-byte reads are served in four parts, the first
+// of lanes 0-3, 12-15 and 20-27).
 template <bool CROSS, int R, int WAVES>
 struct Side {
-  static constexpr int LOADS = R / 16 / WAVES;  // of 1 KB, by a wave and step
+  static constexpr int LOADS = R / 8 / WAVES;  // of 1 KB, by a wave and step
   static constexpr int BYTES = R * STEP;
-  static_assert(LOADS * WAVES * 16 == R, "whole loads");
+  static_assert(LOADS * WAVES * 8 == R, "whole loads");
   const char* base;  // of the workgroup's first row (crosswise: column)
   int64_t ld;
   int count;    // rows there are (crosswise: bytes of a row from the first column on)
-  int at[LOADS], row[LOADS];
+  int at[LOADS], row[LOADS];  // a load's offset, and the row of its step (along: the byte of its row) that it starts at
 
   __device__ __forceinline__ Side(const char* p, int64_t ld_, int first, int total, int lane, int wave) : ld(ld_) {
     if constexpr (CROSS) {
@@ -116,28 +120,30 @@ struct Side {
     } else {
       base = p + (int64_t)first * ld;
       count = total - first < R ? total - first : R;
-      const int piece = (lane & 3) ^ (lane >> 4 & 3);
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        const int r = (wave * LOADS + j) * 16 + (lane >> 2);
+        const int r = (wave * LOADS + j) * 8 + (lane >> 3), piece = (lane & 7) ^ (r >> 1 & 7);
         at[j] = (r < count ? r : count - 1) * (int)ld + piece * 16;
         row[j] = piece * 16;
       }
     }
   }
-  // step k0 / 64 (k0 in bytes of the summed dimension) into `to`; zeros from `end` on
-  __device__ __forceinline__ void load(uint32_t to, int k0, int end, int wave) const {
+  // what the loads of one step share: the step at k0 (in bytes of the summed dimension), zeros from `end` on
+  struct Step {
+    i32x4_t buffer;
+    int k0, left;  // left: rows (crosswise), bytes of a row that there are
+  };
+  __device__ __forceinline__ Step step(int k0, int end) const {
     if constexpr (CROSS) {
-      const int rows = (end - k0) / 2, most = rows < 32 ? rows : 32, have = most > 1 ? most : 1;
-      const i32x4_t r = buffer_of(base + (int64_t)(k0 / 2) * ld, (have - 1) * (int)ld + count);
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) load_to_lds(r, row[j] < rows ? at[j] : -16, to + (wave * LOADS + j) * 1024);
+      const int rows = (end - k0) / 2, most = rows < 64 ? rows : 64, have = most > 1 ? most : 1;
+      return {buffer_of(base + (int64_t)(k0 / 2) * ld, (have - 1) * (int)ld + count), k0, rows};
     } else {
-      const i32x4_t r = buffer_of(base, (count - 1) * (int)ld + ((end + 15) & ~15));
-      const bool in = k0 + row[0] < end;
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) load_to_lds(r, in ? at[j] + k0 : -16, to + (wave * LOADS + j) * 1024);
+      return {buffer_of(base, (count - 1) * (int)ld + ((end + 15) & ~15)), k0, end - k0};
     }
+  }
+  // load j of a step into the slot at `to`
+  __device__ __forceinline__ void load(const Step& s, int j, uint32_t to, int wave) const {
+    load_to_lds(s.buffer, row[j] < s.left ? (CROSS ? at[j] : at[j] + s.k0) : -16, to + (wave * LOADS + j) * 1024);
   }
   // where a lane reads its part of the sixteen rows of C from tile `first` on
   __device__ static __forceinline__ int read_at(int lane, int first) {
@@ -146,35 +152,35 @@ struct Side {
       const int k = 8 * g + (i >> 2), spread = (k & 3) | (k >> 1 & 4);
       return k * (2 * R) + ((first ^ spread) << 5) + (i & 3) * 8;
     } else {
-      return first * 1024 + i * STEP + ((g ^ (i >> 2)) & 3) * 16;
+      return first * (16 * STEP) + i * STEP + (g ^ (i >> 1)) * 16;
     }
   }
-  // tile `first` + i of the step at `from`, where first is a multiple of a power of two above i
-  __device__ static __forceinline__ i32x4_t read(const char* from, int at, int i) {
+  // tile `first` + i of a half of the step at `from`, where first is a multiple of a power of two above i
+  __device__ static __forceinline__ i32x4_t read(const char* from, int at, int i, int half) {
     if constexpr (CROSS) {
       typedef short s4_t __attribute__((ext_vector_type(4)));
-      const auto* p = (__attribute__((address_space(3))) s4_t*)(from + (at ^ (i << 5)));
+      const auto* p = (__attribute__((address_space(3))) s4_t*)(from + half * (64 * R) + (at ^ (i << 5)));
       union {
-        s4_t half[2];
+        s4_t part[2];
         i32x4_t whole;
       } v;
-      v.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p);
-      v.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p + R);  // four rows on
+      v.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p);
+      v.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p + R);  // four rows on
       return v.whole;
     } else {
-      return *(const i32x4_t*)(from + at + i * 1024);
+      return *(const i32x4_t*)(from + (at ^ (half * 64)) + i * (16 * STEP));
     }
   }
 };
 
-template <typename EL, int BM, int BN, int WM, int WN, int S, bool AX = false, bool BX = false>
+template <typename EL, int BM, int BN, int WM, int WN, bool AX = false, bool BX = false>
 struct Gemm {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  static constexpr int SLOT = (BM + BN) * STEP;
-  static constexpr int LDS = S * SLOT;
   typedef Side<AX, BM, WAVES> A;
   typedef Side<BX, BN, WAVES> B;
+  static constexpr int SLOT = A::BYTES > B::BYTES ? A::BYTES : B::BYTES, SLOTS = 5;
+  static constexpr int LDS = SLOTS * SLOT;
   static_assert(!(AX || BX) || !std::is_same<EL, I8>::value, "the transposing read takes 16-bit values");
   static_assert((FM & (FM - 1)) == 0 && (FN & (FN - 1)) == 0 && BM >= 128 && BN >= 128, "what the spread over the banks assumes");
   typedef typename Mma<EL>::acc_t acc_t;
@@ -189,73 +195,125 @@ struct Gemm {
     const A side_a(g.a, g.lda, t.m * BM, g.m, lane, wave);
     const B side_b(g.b, g.ldb, t.n * BN, g.n, lane, wave);
     const uint32_t ring = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-    const auto issue = [&](int step, int slot) {
-      const uint32_t to = ring + slot * SLOT;
-      side_a.load(to, (first + step) * STEP, end, wave);
-      side_b.load(to + BM * STEP, (first + step) * STEP, end, wave);
-    };
     const int wm = wave / WN, wn = wave % WN;
     const int at_a = A::read_at(lane, wm * FM), at_b = B::read_at(lane, wn * FN);
-    const auto a_at = [&](int slot, int i) { return A::read(lds + slot * SLOT, at_a, i); };
-    const auto b_at = [&](int slot, int j) { return B::read(lds + slot * SLOT + BM * STEP, at_b, j); };
+    const auto after = [](int slot, int n) { return slot + n >= SLOTS ? slot + n - SLOTS : slot + n; };
+    const auto load_a = [&](int step, int slot) {
+      const typename A::Step s = side_a.step((first + step) * STEP, end);
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue(s, s);
-    constexpr int L = A::LOADS + B::LOADS;
-    wait_and_meet<(S - 2) * L>();
+      for (int j = 0; j < A::LOADS; ++j) side_a.load(s, j, ring + slot * SLOT, wave);
+    };
+    load_a(0, 0);
+    {
+      const typename B::Step s = side_b.step(first * STEP, end);
+#pragma unroll
+      for (int j = 0; j < B::LOADS; ++j) side_b.load(s, j, ring + SLOT, wave);
+    }
+    load_a(1, 2);
+    {
+      const typename B::Step s = side_b.step((first + 1) * STEP, end);
+#pragma unroll
+      for (int j = 0; j < B::LOADS; ++j) side_b.load(s, j, ring + 3 * SLOT, wave);
+    }
+    wait_and_meet<A::LOADS + B::LOADS>();
     i32x4_t fa[FM], fb[FN], fc[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fa[i] = a_at(0, i);
+    for (int i = 0; i < FM; ++i) fa[i] = A::read(lds, at_a, i, 0);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fb[j] = b_at(0, j);
-    int slot = 0;  // of the step being multiplied
-    // one step: its operands are in registers; those of the next take their place as they are used up
-    const auto turn = [&](int step, const i32x4_t(&now)[FN], i32x4_t(&then)[FN]) {
-      // every wave has its operands of `step` in registers, and step + 1 is in LDS: the slot before `slot` is free
-      wait_and_meet<(S - 3) * L>();
-      issue(step + S - 1, slot == 0 ? S - 1 : slot - 1);
-      slot = slot + 1 == S ? 0 : slot + 1;
+    for (int j = 0; j < FN; ++j) fb[j] = B::read(lds + SLOT, at_b, j, 0);
+    // One half of a step: its operands are in registers; those of the next half (from the slots at a and b) take their place as they are used up,
+    // and `load` sends the loads that fall into this half, one behind each of its first rows of tiles.  (All of them at once, behind the meeting,
+    // queue up in front of the matrix instructions.)  The last row's operand moves aside, so that the last read is a row old when the half ends.
+    const auto half = [&](const i32x4_t(&now)[FN], i32x4_t(&then)[FN], const char* a, const char* b, int h, auto&& load, int loads) {
+      const i32x4_t last = fa[FM - 1];
+      fa[FM - 1] = A::read(a, at_a, FM - 1, h);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = Mma<EL>::run(now[j], fa[i], acc[i][j]);
-        fa[i] = a_at(slot, i);
+        for (int j = 0; j < FN; ++j) acc[i][j] = Mma<EL>::run(now[j], i < FM - 1 ? fa[i] : last, acc[i][j]);
+        if (i < FM - 1) fa[i] = A::read(a, at_a, i, h);
 #pragma unroll
-        for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) then[j] = b_at(slot, j);
-        __builtin_amdgcn_sched_barrier(0);  // the reads stay here, a step ahead of their use
+        for (int j = i * FN / (FM - 1); j < (i + 1) * FN / (FM - 1) && j < FN; ++j) then[j] = B::read(b, at_b, j, h);
+#pragma unroll
+        for (int j = i * PER_ROW; j < (i + 1) * PER_ROW; ++j)
+          if (j < loads) load(j);
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay here, half a step ahead of their use
       }
     };
-    for (int step = 0; step < steps; step += 2) {  // an odd number of steps ends with one of zeros
-      turn(step, fb, fc);
-      turn(step + 1, fc, fb);
+    int slot = 0;  // of A's step; B's is the next one
+    for (int step = 0; step < steps; ++step) {
+      const int a1 = after(slot, 2), b1 = after(slot, 3), b0 = after(slot, 1);
+      {
+        // A of the step after the next goes where B of the last step was
+        const typename A::Step s = side_a.step((first + step + 2) * STEP, end);
+        const uint32_t to = ring + after(slot, 4) * SLOT;
+        half(fb, fc, lds + slot * SLOT, lds + b0 * SLOT, 1, [&](int j) { side_a.load(s, j, to, wave); }, A::LOADS);
+      }
+      wait_and_meet<A::LOADS>();
+      {
+        // B of it where A of this step was
+        const typename B::Step s = side_b.step((first + step + 2) * STEP, end);
+        const uint32_t to = ring + slot * SLOT;
+        half(fc, fb, lds + a1 * SLOT, lds + b1 * SLOT, 0, [&](int j) { side_b.load(s, j, to, wave); }, B::LOADS);
+      }
+      slot = a1;
     }
     wait_and_meet<0>();  // nothing may still be on its way to LDS when it is used again, or at the workgroup's end
   }
 
-  // all but the last LEFT loads of this wave are in LDS, its reads are done, and so are the other waves'
+  static constexpr int PER_ROW = (A::LOADS + FM - 1) / FM > (B::LOADS + FM - 1) / FM ? (A::LOADS + FM - 1) / FM : (B::LOADS + FM - 1) / FM;
+
+  // all but the last LEFT loads of this wave are in LDS, all of its reads are done, and so for the other waves
   template <int LEFT>
   __device__ static __forceinline__ void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
   }
 };
 
+// Four neighbouring values of a row that has `left` of them from here on, stored from any address of their type.
+template <typename YT>
+__device__ __forceinline__ void store4(typename YT::storage* o, int left, const float (&v)[4]) {
+  if constexpr (std::is_same<YT, F32>::value) {
+    if (left >= 4) __builtin_memcpy(o, v, 16);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = v[i];
+  } else {
+    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
+    if (left >= 4) __builtin_memcpy(o, w, 8);
+    else
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+  }
+}
+// p[n .. n + 3] of a vector of `count` (n below it) as float32; behind the end its first of the four again
+__device__ __forceinline__ void load4(const void* p, int dt, int n, int count, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = load_as_f32(p, n + i < count ? n + i : n, dt);
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
 // whether rows of `bytes` with `ld` bytes between them can be read as they are; 256 of them stay inside 31 bits
 inline bool rows_fit(const void* p, int64_t ld, int64_t bytes) { return bytes % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
 
-// Tiles of 256 x 256 where there are enough of them for the chip, else of 128 x 128, with the summed dimension in runs of at least
-// eight steps so that some 512 workgroups come together.
+// Tiles of 256 x 256, one to a compute unit, or of 128 x 128, two to one (two take 0.57 of the time of a large one, one alone 0.33): what needs
+// less for all of them.  Where even the small ones leave compute units idle the summed dimension is cut into runs of at least four steps.
 struct TilePlan {
   int bm, splits, split_steps;
   int64_t slot_bytes;
 };
 inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
+  constexpr int64_t CUS = 256;
   TilePlan p{};
-  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-  p.bm = big >= 192 ? 256 : 128;
-  const int64_t tiles = p.bm == 256 ? big : small, steps = (kbytes + STEP - 1) / STEP;
-  int64_t splits = p.bm == 256 ? 1 : 512 / tiles;
-  if (splits > steps / 8) splits = steps / 8;
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128), last = small % (2 * CUS);
+  const double cost_big = (double)((big + CUS - 1) / CUS), cost_small = 0.57 * (double)(small / (2 * CUS)) + (last == 0 ? 0.0 : last <= CUS ? 0.33 : 0.57);
+  p.bm = cost_big <= cost_small ? 256 : 128;
+  const int64_t steps = (kbytes + STEP - 1) / STEP;
+  int64_t splits = p.bm == 256 ? 1 : 2 * CUS / small;
+  if (splits > steps / 4) splits = steps / 4;
   if (splits < 1) splits = 1;
   p.split_steps = (int)((steps + splits - 1) / splits);
   p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);

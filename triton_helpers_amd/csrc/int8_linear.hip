@@ -19,31 +19,18 @@ struct Epilogue {
   int bias_dt, y_dt, act, m, n;
 };
 
+// four columns of a row: s the row's scale, t and b the columns' (zeros without a bias)
 template <int ACT, typename YT>
-__device__ __forceinline__ void put4(const Epilogue& e, int m, int n, const int (&sum)[4], float s) {
-  const int left = e.n - n;
+__device__ __forceinline__ void put4(const Epilogue& e, int m, int n, const int (&sum)[4], float s, const float (&t)[4], const float (&b)[4]) {
   float v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = i < left ? n + i : n;
-    const float z = (float)sum[i] * (s * e.t[c]);
-    v[i] = act_value<ACT>(e.bias == nullptr ? z : z + load_as_f32(e.bias, c, e.bias_dt));
-  }
-  auto* o = (typename YT::storage*)e.y + (int64_t)m * e.ldy + n;
-  if constexpr (std::is_same<YT, F32>::value) {
-    if (left >= 4) __builtin_memcpy(o, v, 16);
-    else
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = v[i];
-  } else {
-    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
-    if (left >= 4) __builtin_memcpy(o, w, 8);
-    else
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-  }
+  for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(fmaf((float)sum[i], s * t[i], b[i]));
+  store4<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, v);
+}
+__device__ __forceinline__ void columns4(const Epilogue& e, int n, float (&t)[4], float (&b)[4]) {
+  load4(e.t, NF_F32, n, e.n, t);
+  if (e.bias != nullptr) load4(e.bias, e.bias_dt, n, e.n, b);
+  else b[0] = b[1] = b[2] = b[3] = 0.0f;
 }
 
 // body(activation, type of y) under one branch that is the same for every thread
@@ -144,8 +131,10 @@ __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
     for (int v = 0; v < W; ++v)
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] += part[v][tile][c][from];
+    float t[4], b[4];
+    columns4(a.e, n, t, b);
     const float s = a.e.s[m];
-    with_epilogue(a.e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s); });
+    with_epilogue(a.e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s, t, b); });
   }
 }
 
@@ -170,17 +159,22 @@ __global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogu
       }
     return;
   }
+  // everything that the results are scaled with is asked for at once
+  float s[G::FM], tn[G::FN][4], bn[G::FN][4];
+#pragma unroll
+  for (int i = 0; i < G::FM; ++i) s[i] = e.s[m0 + 16 * i < g.m ? m0 + 16 * i : g.m - 1];
+#pragma unroll
+  for (int j = 0; j < G::FN; ++j) columns4(e, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1, tn[j], bn[j]);
   with_epilogue(e, [&](auto act_c, auto y_c) {
 #pragma unroll
     for (int i = 0; i < G::FM; ++i) {
       const int m = m0 + 16 * i;
       if (m >= g.m) continue;
-      const float s = e.s[m];
 #pragma unroll
       for (int j = 0; j < G::FN; ++j) {
         const int n = n0 + 16 * j;
         const int sum[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (n < g.n) put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s);
+        if (n < g.n) put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s[i], tn[j], bn[j]);
       }
     }
   });
@@ -194,8 +188,10 @@ __global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, 
   i32x4_t v = {0, 0, 0, 0};
   for (int k = 0; k < splits; ++k) v += *(const i32x4_t*)(slots + k * each + (int64_t)m * ld + n);
   const int sum[4] = {v[0], v[1], v[2], v[3]};
+  float t[4], b[4];
+  columns4(e, n, t, b);
   const float s = e.s[m];
-  with_epilogue(e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s); });
+  with_epilogue(e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s, t, b); });
 }
 
 // rows copied to 16-byte boundaries and filled up with zeros, 16 bytes a thread
@@ -233,9 +229,9 @@ Plan plan(const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t m, int
   return p;
 }
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN>
 int tile_launch(GemmArgs g, const Epilogue& e, int* slots, hipStream_t s) {
-  typedef Gemm<I8, BM, BN, WM, WN, S> G;
+  typedef Gemm<I8, BM, BN, WM, WN> G;
   g.tiles_m = (g.m + BM - 1) / BM;
   g.tiles_n = (g.n + BN - 1) / BN;
   hipLaunchKernelGGL((int8_tile_k<G, BM, BN, WM, WN>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e, slots);
@@ -294,7 +290,7 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   }
   const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)k, 0, 0, p.tile.splits, p.tile.split_steps};
   int* slots = p.tile.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
-  const int rc = p.tile.bm == 256 ? tile_launch<256, 256, 2, 4, 4>(g, e, slots, s) : tile_launch<128, 128, 2, 2, 4>(g, e, slots, s);
+  const int rc = p.tile.bm == 256 ? tile_launch<256, 256, 4, 2>(g, e, slots, s) : tile_launch<128, 128, 2, 2>(g, e, slots, s);
   if (rc != 0 || slots == nullptr) return rc;
   hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.tile.splits, e);
   return check_launch("int8_sum");
