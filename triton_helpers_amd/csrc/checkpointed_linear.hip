@@ -30,29 +30,26 @@ __device__ __forceinline__ float gated(float v, float x) {
   else return v * act_slope<ACT>(x);
 }
 
-// four values of the gate's rows; a NaN scale stays one
-__device__ __forceinline__ int gate4(const Out& e, int m, int n) {
-  const int8_t* q = e.q + (int64_t)m * e.n + n;
-  int8_t c[4];
-  const int left = e.n - n;
-  if (left >= 4) __builtin_memcpy(c, q, 4);
-  else
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = q[i < left ? i : 0];
-  return __builtin_bit_cast(int, c);
-}
-
-// four columns of a row: b the columns' biases; q, s the gate's values and scale
+// eight columns of a row; b: their biases
 template <int MODE, int ACT, typename YT>
-__device__ __forceinline__ void put4(const Out& e, int m, int n, f32x4_t v, const float (&b)[4], int q, float s) {
-  float r[4];
+__device__ __forceinline__ void put8(const Out& e, int m, int n, const float (&v)[8], const float (&b)[8]) {
+  const int left = e.n - n;
+  float r[8];
+  if constexpr (MODE == OUT_GATE && ACT != NF_ACT_NONE) {
+    const int8_t* q = e.q + (int64_t)m * e.n + n;
+    int8_t c[8];
+    if (left >= 8) __builtin_memcpy(c, q, 8);
+    else
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (MODE == OUT_BIAS) r[i] = v[i] + b[i];
-    else if constexpr (MODE == OUT_GATE) r[i] = gated<ACT>(v[i], s * (float)(q << (24 - 8 * i) >> 24));
-    else r[i] = v[i];
+      for (int i = 0; i < 8; ++i) c[i] = q[i < left ? i : 0];
+    const float s = e.s[m];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = gated<ACT>(v[i], s * (float)c[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = MODE == OUT_BIAS ? v[i] + b[i] : v[i];
   }
-  store4<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, r);
+  store8<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, left, r);
 }
 
 // body(activation, type of y) under branches that are the same for every thread
@@ -64,73 +61,45 @@ __device__ __forceinline__ void with_out(const Out& e, Body&& body) {
   else body(Int<NF_ACT_NONE>{}, T{});
 }
 
-template <typename T, typename G, int BM, int BN, int WM, int WN, int MODE>
+template <typename T, typename G, int MODE>
 __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, float* slots) {
   __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
   f32x4_t acc[G::FM][G::FN] = {};
   const Tile t = tile_of(g, blockIdx.x);
   G::run(g, t, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = t.m * BM + wave / WN * (BM / WM) + (lane & 15), n0 = t.n * BN + wave % WN * (BN / WN) + (lane >> 4) * 4;
-  if (slots != nullptr) {  // [split][m][n rounded up to 4]
-    const int64_t ld = (g.n + 3) / 4 * 4;
-    float* o = slots + (int64_t)t.split * g.m * ld;
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i)
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j) {
-        const int m = m0 + 16 * i, n = n0 + 16 * j;
-        if (m < g.m && n < g.n) *(f32x4_t*)(o + (int64_t)m * ld + n) = acc[i][j];
-      }
+  const int n = G::column(t);
+  if (slots != nullptr) {  // [split][m][n rounded up to 8]
+    const int64_t ld = (g.n + 7) / 8 * 8;
+    float* o = slots + (int64_t)t.split * g.m * ld + n;
+    G::each8(t, lds, acc, [&](int m, const float (&v)[8]) {
+      if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+    });
     return;
   }
-  // what the results go together with is asked for at once
-  float b[G::FN][4] = {}, s[G::FM] = {};
-  int q[G::FM][G::FN] = {};
-  if (MODE == OUT_BIAS && e.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < G::FN; ++j) load4(e.bias, e.bias_dt, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1, g.n, b[j]);
-  }
-  if (MODE == OUT_GATE && e.act != NF_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i) {
-      const int m = m0 + 16 * i < g.m ? m0 + 16 * i : g.m - 1;
-      s[i] = e.s[m];
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j) q[i][j] = gate4(e, m, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1);
-    }
-  }
+  float b[8] = {};
+  if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
   with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i) {
-      const int m = m0 + 16 * i;
-      if (m >= g.m) continue;
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j) {
-        const int n = n0 + 16 * j;
-        if (n < g.n) put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, acc[i][j], b[j], q[i][j], s[i]);
-      }
-    }
+    G::each8(t, lds, acc, [&](int m, const float (&v)[8]) {
+      if (m < g.m && n < g.n) put8<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b);
+    });
   });
 }
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits, Out e) {
-  const int64_t quads = (e.n + 3) / 4, ld = quads * 4, each = (int64_t)e.m * ld;
+  const int64_t parts = (e.n + 7) / 8, ld = parts * 8, each = (int64_t)e.m * ld;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= e.m * quads) return;
-  const int m = (int)(at / quads), n = (int)(at % quads) * 4;
-  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (at >= e.m * parts) return;
+  const int m = (int)(at / parts), n = (int)(at % parts) * 8;
+  float v[8] = {}, b[8] = {};
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) v += *(const f32x4_t*)(slots + k * each + (int64_t)m * ld + n);
-  float b[4] = {}, s = 0.0f;
-  int q = 0;
-  if (MODE == OUT_BIAS && e.bias != nullptr) load4(e.bias, e.bias_dt, n, e.n, b);
-  if (MODE == OUT_GATE && e.act != NF_ACT_NONE) {
-    q = gate4(e, m, n);
-    s = e.s[m];
+  for (int k = 0; k < splits; ++k) {
+    const float* p = slots + k * each + (int64_t)m * ld + n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += p[i];
   }
-  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put4<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b, q, s); });
+  if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
+  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put8<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b); });
 }
 
 // act(s q) in 16 bits, rows filled up with zeros to whole 16-byte pieces; a stream, eight values a thread
@@ -191,7 +160,7 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
     typedef Gemm<T, B, B, WM, WN, AX, BX> G;
     g.tiles_m = (g.m + B - 1) / B;
     g.tiles_n = (g.n + B - 1) / B;
-    hipLaunchKernelGGL((keep_tile_k<T, G, B, B, WM, WN, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
+    hipLaunchKernelGGL((keep_tile_k<T, G, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
                        p.splits > 1 ? slots : nullptr);
   };
   // (waves of 64 x 128 are 2 % quicker than 128 x 64 where both operands lie along the sum, 2 to 5 % slower where one is crosswise)
@@ -200,7 +169,7 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
   else go(Int<256>{}, Int<4>{}, Int<2>{});
   const int rc = check_launch("checkpointed_linear");
   if (rc != 0 || p.splits == 1) return rc;
-  hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
+  hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 7) / 8) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
   return check_launch("checkpointed_linear_sum");
 }
 

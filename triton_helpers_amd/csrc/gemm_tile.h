@@ -261,6 +261,36 @@ struct Gemm {
     wait_and_meet<0>();  // nothing may still be on its way to LDS when it is used again, or at the workgroup's end
   }
 
+  // The sums in rows: body(m, v) for eight neighbouring columns from column() on, each row of the wave's part once, behind run().  They
+  // go through LDS, so that a row leaves in whole cache lines and the code behind them is one short loop (unrolled over the tiles it
+  // costs a small product more in instruction fetches than its sums).
+  static constexpr int LPR = 2 * FN;  // lanes to a row
+  __device__ static __forceinline__ int column(const Tile& t) {
+    return t.n * BN + (int)(threadIdx.x >> 6) % WN * (BN / WN) + (int)(threadIdx.x & 63) % LPR * 8;
+  }
+  template <typename Acc, typename Body>
+  __device__ static __forceinline__ void each8(const Tile& t, char* lds, const Acc (&acc)[FM][FN], Body&& body) {
+    typedef typename std::remove_cv<typename std::remove_reference<decltype(acc[0][0][0])>::type>::type E;
+    constexpr int LD = 16 * FN + 4, PASSES = 16 * FM * LD * 4 * WAVES <= LDS ? 1 : 2, ROWS = 16 * FM / PASSES;
+    static_assert(ROWS * LD * 4 * WAVES <= LDS, "a strip for every wave");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m0 = t.m * BM + wave / WN * (BM / WM);
+    E* strip = (E*)lds + wave * (ROWS * LD);
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+#pragma unroll
+      for (int i = 0; i < FM / PASSES; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) *(Acc*)(strip + (16 * i + (lane & 15)) * LD + 16 * j + 4 * (lane >> 4)) = acc[p * (FM / PASSES) + i][j];
+#pragma unroll 2
+      for (int r = lane / LPR; r < ROWS; r += 64 / LPR) {
+        E v[8];
+        *(Acc*)v = *(const Acc*)(strip + r * LD + lane % LPR * 8);
+        *(Acc*)(v + 4) = *(const Acc*)(strip + r * LD + lane % LPR * 8 + 4);
+        body(m0 + p * ROWS + r, v);
+      }
+    }
+  }
+
   static constexpr int PER_ROW = (A::LOADS + FM - 1) / FM > (B::LOADS + FM - 1) / FM ? (A::LOADS + FM - 1) / FM : (B::LOADS + FM - 1) / FM;
 
   // all but the last LEFT loads of this wave are in LDS, all of its reads are done, and so for the other waves
@@ -270,28 +300,10 @@ struct Gemm {
   }
 };
 
-// Four neighbouring values of a row that has `left` of them from here on, stored from any address of their type.
-template <typename YT>
-__device__ __forceinline__ void store4(typename YT::storage* o, int left, const float (&v)[4]) {
-  if constexpr (std::is_same<YT, F32>::value) {
-    if (left >= 4) __builtin_memcpy(o, v, 16);
-    else
+// p[n .. n + 7] of a vector of `count` as float32; zeros behind its end
+__device__ __forceinline__ void vector8(const void* p, int dt, int n, int count, float (&v)[8]) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = v[i];
-  } else {
-    const uint32_t w[2] = {YT::pack(v[0], v[1]), YT::pack(v[2], v[3])};
-    if (left >= 4) __builtin_memcpy(o, w, 8);
-    else
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < left) o[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-  }
-}
-// p[n .. n + 3] of a vector of `count` (n below it) as float32; behind the end its first of the four again
-__device__ __forceinline__ void load4(const void* p, int dt, int n, int count, float (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = load_as_f32(p, n + i < count ? n + i : n, dt);
+  for (int i = 0; i < 8; ++i) v[i] = n + i < count ? load_as_f32(p, n + i, dt) : 0.0f;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -317,7 +329,7 @@ inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
   if (splits < 1) splits = 1;
   p.split_steps = (int)((steps + splits - 1) / splits);
   p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
-  if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 4) * 4, 256);
+  if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 8) * 4, 256);
   return p;
 }
 // copies rows to 16-byte boundaries, filled up with zeros to whole 16-byte pieces (int8_linear.hip)

@@ -19,18 +19,24 @@ struct Epilogue {
   int bias_dt, y_dt, act, m, n;
 };
 
-// four columns of a row: s the row's scale, t and b the columns' (zeros without a bias)
-template <int ACT, typename YT>
-__device__ __forceinline__ void put4(const Epilogue& e, int m, int n, const int (&sum)[4], float s, const float (&t)[4], const float (&b)[4]) {
-  float v[4];
+// What eight columns share: their scales and biases (zeros without any).
+struct Columns {
+  float t[8], b[8];
+  __device__ __forceinline__ Columns(const Epilogue& e, int n) {
+    vector8(e.t, NF_F32, n, e.n, t);
+    if (e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
+    else
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(fmaf((float)sum[i], s * t[i], b[i]));
-  store4<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, v);
-}
-__device__ __forceinline__ void columns4(const Epilogue& e, int n, float (&t)[4], float (&b)[4]) {
-  load4(e.t, NF_F32, n, e.n, t);
-  if (e.bias != nullptr) load4(e.bias, e.bias_dt, n, e.n, b);
-  else b[0] = b[1] = b[2] = b[3] = 0.0f;
+      for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+  }
+};
+// eight columns of a row, whose scale is s
+template <int ACT, typename YT>
+__device__ __forceinline__ void put8(const Epilogue& e, int m, int n, const int (&sum)[8], float s, const Columns& c) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = act_value<ACT>(fmaf((float)sum[i], s * c.t[i], c.b[i]));
+  store8<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, v);
 }
 
 // body(activation, type of y) under one branch that is the same for every thread
@@ -120,78 +126,60 @@ __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) part[wave][i * NT + j][c][lane] = acc[i][j][c];
   __syncthreads();
-  // a thread adds up four neighbouring columns of a row: lane and numbers as the matrix instruction left them
-  for (int at = threadIdx.x; at < MT * NT * 64; at += 64 * W) {
-    const int j = at % (4 * NT), m = at / (4 * NT);  // four columns 4 j, row m
-    const int from = (j & 3) * 16 + (m & 15), tile = (m >> 4) * NT + (j >> 2);
-    const int n = n0 + 4 * j;
+  // a thread adds up eight neighbouring columns of a row: lane and numbers as the matrix instruction left them
+  for (int at = threadIdx.x; at < MT * NT * 32; at += 64 * W) {
+    const int j = at % (2 * NT), m = at / (2 * NT), n = n0 + 8 * j;  // columns 8 j.. of row m
     if (m >= a.e.m || n >= a.e.n) continue;
-    int sum[4] = {};
+    const Columns columns(a.e, n);
+    const float s = a.e.s[m];
+    const int from = (j & 1) * 32 + (m & 15), tile = (m >> 4) * NT + (j >> 1);
+    int sum[8] = {};
 #pragma unroll
     for (int v = 0; v < W; ++v)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sum[c] += part[v][tile][c][from];
-    float t[4], b[4];
-    columns4(a.e, n, t, b);
-    const float s = a.e.s[m];
-    with_epilogue(a.e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s, t, b); });
+      for (int c = 0; c < 8; ++c) sum[c] += part[v][tile][c & 3][from + (c >> 2) * 16];
+    with_epilogue(a.e, [&](auto act_c, auto y_c) { put8<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s, columns); });
   }
 }
 
 // ---- tiles --------------------------------------------------------------------------------------
-template <typename G, int BM, int BN, int WM, int WN>
+template <typename G>
 __global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogue e, int* slots) {
   __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
   i32x4_t acc[G::FM][G::FN] = {};
   const Tile t = tile_of(g, blockIdx.x);
   G::run(g, t, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = t.m * BM + wave / WN * (BM / WM) + (lane & 15), n0 = t.n * BN + wave % WN * (BN / WN) + (lane >> 4) * 4;
-  if (slots != nullptr) {  // [split][m][n rounded up to 4]
-    const int64_t ld = (g.n + 3) / 4 * 4;
-    int* o = slots + (int64_t)t.split * g.m * ld;
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i)
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j) {
-        const int m = m0 + 16 * i, n = n0 + 16 * j;
-        if (m < g.m && n < g.n) *(i32x4_t*)(o + (int64_t)m * ld + n) = acc[i][j];
-      }
+  const int n = G::column(t);
+  if (slots != nullptr) {  // [split][m][n rounded up to 8]
+    const int64_t ld = (g.n + 7) / 8 * 8;
+    int* o = slots + (int64_t)t.split * g.m * ld + n;
+    G::each8(t, lds, acc, [&](int m, const int (&v)[8]) {
+      if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+    });
     return;
   }
-  // everything that the results are scaled with is asked for at once
-  float s[G::FM], tn[G::FN][4], bn[G::FN][4];
-#pragma unroll
-  for (int i = 0; i < G::FM; ++i) s[i] = e.s[m0 + 16 * i < g.m ? m0 + 16 * i : g.m - 1];
-#pragma unroll
-  for (int j = 0; j < G::FN; ++j) columns4(e, n0 + 16 * j < g.n ? n0 + 16 * j : g.n - 1, tn[j], bn[j]);
+  const Columns columns(e, n);
   with_epilogue(e, [&](auto act_c, auto y_c) {
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i) {
-      const int m = m0 + 16 * i;
-      if (m >= g.m) continue;
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j) {
-        const int n = n0 + 16 * j;
-        const int sum[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (n < g.n) put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s[i], tn[j], bn[j]);
-      }
-    }
+    G::each8(t, lds, acc, [&](int m, const int (&v)[8]) {
+      if (m < g.m && n < g.n) put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, v, e.s[m], columns);
+    });
   });
 }
 
 __global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, Epilogue e) {
-  const int64_t quads = (e.n + 3) / 4, ld = quads * 4, each = (int64_t)e.m * ld;
+  const int64_t parts = (e.n + 7) / 8, ld = parts * 8, each = (int64_t)e.m * ld;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= e.m * quads) return;
-  const int m = (int)(at / quads), n = (int)(at % quads) * 4;
-  i32x4_t v = {0, 0, 0, 0};
-  for (int k = 0; k < splits; ++k) v += *(const i32x4_t*)(slots + k * each + (int64_t)m * ld + n);
-  const int sum[4] = {v[0], v[1], v[2], v[3]};
-  float t[4], b[4];
-  columns4(e, n, t, b);
+  if (at >= e.m * parts) return;
+  const int m = (int)(at / parts), n = (int)(at % parts) * 8;
+  int sum[8] = {};
+  for (int k = 0; k < splits; ++k) {
+    const int* p = slots + k * each + (int64_t)m * ld + n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += p[i];
+  }
+  const Columns columns(e, n);
   const float s = e.s[m];
-  with_epilogue(e, [&](auto act_c, auto y_c) { put4<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s, t, b); });
+  with_epilogue(e, [&](auto act_c, auto y_c) { put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s, columns); });
 }
 
 // rows copied to 16-byte boundaries and filled up with zeros, 16 bytes a thread
@@ -234,7 +222,7 @@ int tile_launch(GemmArgs g, const Epilogue& e, int* slots, hipStream_t s) {
   typedef Gemm<I8, BM, BN, WM, WN> G;
   g.tiles_m = (g.m + BM - 1) / BM;
   g.tiles_n = (g.n + BN - 1) / BN;
-  hipLaunchKernelGGL((int8_tile_k<G, BM, BN, WM, WN>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e, slots);
+  hipLaunchKernelGGL((int8_tile_k<G>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e, slots);
   return check_launch("int8_linear");
 }
 
@@ -292,6 +280,6 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   int* slots = p.tile.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
   const int rc = p.tile.bm == 256 ? tile_launch<256, 256, 4, 2>(g, e, slots, s) : tile_launch<128, 128, 2, 2>(g, e, slots, s);
   if (rc != 0 || slots == nullptr) return rc;
-  hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 3) / 4) + 255) / 256)), dim3(256), 0, s, slots, p.tile.splits, e);
+  hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 7) / 8) + 255) / 256)), dim3(256), 0, s, slots, p.tile.splits, e);
   return check_launch("int8_sum");
 }
