@@ -20,6 +20,9 @@ struct Out {
   const int8_t* q;  // the gate's rows, without gaps
   const float* s;
   int m, n, y_dt;
+  float* sums;  // dW: partial sums of dy's columns [split][m], NULL where they are not wanted
+  void* db;     // ... or, of a single run, where they go, in type db_dt
+  int db_dt;
 };
 
 // v * act'(x^); a closed gate lets nothing through, not even an infinity
@@ -30,26 +33,41 @@ __device__ __forceinline__ float gated(float v, float x) {
   else return v * act_slope<ACT>(x);
 }
 
+// the gate of eight columns of a row
+struct Gate {
+  int q[2];
+  float s;
+};
+template <int ACT>
+__device__ __forceinline__ Gate gate_of(const Out& e, int m, int n) {
+  Gate g{};
+  if constexpr (ACT != NF_ACT_NONE) {
+    if (m < e.m && n < e.n) {
+      const int8_t* q = e.q + (int64_t)m * e.n + n;
+      const int left = e.n - n;
+      if (left >= 8) {
+        __builtin_memcpy(g.q, q, 8);
+      } else {
+        int8_t c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = q[i < left ? i : 0];
+        __builtin_memcpy(g.q, c, 8);
+      }
+      g.s = e.s[m];
+    }
+  }
+  return g;
+}
 // eight columns of a row; b: their biases
 template <int MODE, int ACT, typename YT>
-__device__ __forceinline__ void put8(const Out& e, int m, int n, const float (&v)[8], const float (&b)[8]) {
-  const int left = e.n - n;
+__device__ __forceinline__ void put8(const Out& e, int m, int n, const float (&v)[8], const float (&b)[8], const Gate& g) {
   float r[8];
-  if constexpr (MODE == OUT_GATE && ACT != NF_ACT_NONE) {
-    const int8_t* q = e.q + (int64_t)m * e.n + n;
-    int8_t c[8];
-    if (left >= 8) __builtin_memcpy(c, q, 8);
-    else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = q[i < left ? i : 0];
-    const float s = e.s[m];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = gated<ACT>(v[i], s * (float)c[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = MODE == OUT_BIAS ? v[i] + b[i] : v[i];
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (MODE == OUT_GATE) r[i] = gated<ACT>(v[i], g.s * (float)(g.q[i / 4] << (24 - i % 4 * 8) >> 24));
+    else r[i] = MODE == OUT_BIAS ? v[i] + b[i] : v[i];
   }
-  store8<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, left, r);
+  store8<YT>((typename YT::storage*)e.y + (int64_t)m * e.ldy + n, e.n - n, r);
 }
 
 // body(activation, type of y) under branches that are the same for every thread
@@ -66,12 +84,33 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
   __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
   f32x4_t acc[G::FM][G::FN] = {};
   const Tile t = tile_of(g, blockIdx.x);
-  G::run(g, t, lds, acc);
+  if constexpr (MODE == OUT_PLAIN && G::ROWS_M == 128) {
+    // db on the way: the first column of tiles holds each value of dy once; one of the waves that share a row of them adds it up.  (The sums
+    // take instructions of every wave: nothing in the small tiles, which wait for memory, but 40 % in the large ones.)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool summing = e.sums != nullptr && t.n == 0 && wave % G::WAVES_N == 0;
+    float sums[G::FM] = {};
+    G::template run<true>(g, t, lds, acc, sums);
+    if (summing) {
+      const int m = t.m * G::ROWS_M + wave / G::WAVES_N * (16 * G::FM) + lane;
+#pragma unroll
+      for (int i = 0; i < G::FM; ++i) {
+        float v = sums[i] + __shfl_xor(sums[i], 16);
+        v += __shfl_xor(v, 32);
+        if (lane < 16 && m + 16 * i < g.m) {
+          if (e.db != nullptr) store_any(e.db, m + 16 * i, e.db_dt, v);
+          else e.sums[(int64_t)t.split * g.m + m + 16 * i] = v;
+        }
+      }
+    }
+  } else {
+    G::run(g, t, lds, acc);
+  }
   const int n = G::column(t);
   if (slots != nullptr) {  // [split][m][n rounded up to 8]
     const int64_t ld = (g.n + 7) / 8 * 8;
     float* o = slots + (int64_t)t.split * g.m * ld + n;
-    G::each8(t, lds, acc, [&](int m, const float (&v)[8]) {
+    G::each8(t, lds, acc, [](int) { return 0; }, [&](int m, const float (&v)[8], int) {
       if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
     });
     return;
@@ -79,8 +118,9 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
   float b[8] = {};
   if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
   with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
-    G::each8(t, lds, acc, [&](int m, const float (&v)[8]) {
-      if (m < g.m && n < g.n) put8<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b);
+    constexpr int ACT = decltype(act_c)::value;
+    G::each8(t, lds, acc, [&](int m) { return gate_of<MODE == OUT_GATE ? ACT : NF_ACT_NONE>(e, m, n); }, [&](int m, const float (&v)[8], const Gate& gate) {
+      if (m < g.m && n < g.n) put8<MODE, ACT, decltype(y_c)>(e, m, n, v, b, gate);
     });
   });
 }
@@ -99,7 +139,10 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
     for (int i = 0; i < 8; ++i) v[i] += p[i];
   }
   if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
-  with_out<MODE, T>(e, [&](auto act_c, auto y_c) { put8<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b); });
+  with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    put8<MODE, ACT, decltype(y_c)>(e, m, n, v, b, gate_of<MODE == OUT_GATE ? ACT : NF_ACT_NONE>(e, m, n));
+  });
 }
 
 // act(s q) in 16 bits, rows filled up with zeros to whole 16-byte pieces; a stream, eight values a thread
@@ -194,6 +237,7 @@ KeepFwd keep_fwd(const void* x, int64_t xs, const void* w, int64_t ws, int64_t r
 struct KeepBwd {
   int64_t ldk, ldn, dy_bytes, w_bytes, h_bytes, sum_bytes;
   int strips, groups;
+  bool sums_in_dw;
   TilePlan dx, dw;
   int64_t slots() const { return dx.slot_bytes > dw.slot_bytes ? dx.slot_bytes : dw.slot_bytes; }
   int64_t total() const { return dy_bytes + w_bytes + h_bytes + sum_bytes + slots(); }
@@ -211,7 +255,10 @@ KeepBwd keep_bwd(const void* dy, int64_t dys, const void* w, int64_t ws, int64_t
     p.h_bytes = round_up(rows * p.ldk * 2, 256);
     p.dw = tile_plan(n, k, rows * 2);
   }
-  if (need_db) {
+  p.sums_in_dw = need_db && need_dw && p.dw.bm == 128;
+  if (p.sums_in_dw) {
+    if (p.dw.splits > 1) p.sum_bytes = round_up((int64_t)p.dw.splits * n * 4, 256);
+  } else if (need_db) {
     p.strips = (int)((n + 255) / 256);
     const int64_t most = 1024 / p.strips + 1, want = (rows + 63) / 64;
     p.groups = (int)(want < most ? want : most);
@@ -232,7 +279,7 @@ int fwd(const KeepFwd& p, const void* x, int64_t xs, const void* w, int64_t ws, 
     if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed, n, s)) return rc;
   const GemmArgs g{p.h_bytes > 0 ? h : (const char*)x, p.w_bytes > 0 ? packed : (const char*)w, (p.h_bytes > 0 ? p.ldh : xs) * 2,
                    (p.w_bytes > 0 ? p.ldh : ws) * 2, (int)rows, (int)n, (int)k * 2, 0, 0, 0, 0};
-  const Out e{y, ys, bias, bias_dt, NF_ACT_NONE, nullptr, nullptr, (int)rows, (int)n, T::code};
+  const Out e{y, ys, bias, bias_dt, NF_ACT_NONE, nullptr, nullptr, (int)rows, (int)n, T::code, nullptr, nullptr, 0};
   return product<T, OUT_BIAS, false, false>(g, p.tile, e, slots, s);
 }
 
@@ -241,7 +288,7 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
         void* db, int db_dt, int64_t rows, int64_t n, int64_t k, int act, char* at, hipStream_t s) {
   char *packed_dy = at, *packed_w = packed_dy + p.dy_bytes, *h = packed_w + p.w_bytes, *sums = h + p.h_bytes;
   float* slots = (float*)(sums + p.sum_bytes);
-  if (db != nullptr) {
+  if (db != nullptr && !p.sums_in_dw) {
     hipLaunchKernelGGL((column_sums_k<T>), dim3(p.strips, p.groups), dim3(256), 0, s, (const uint16_t*)dy, dys, rows, (int)n, (float*)sums);
     if (const int rc = check_launch("column_sums")) return rc;
     if (const int rc = sum_slots((const float*)sums, p.groups, n, db, db_dt, s)) return rc;
@@ -257,7 +304,7 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
     if (p.w_bytes > 0)
       if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed_w, n, s)) return rc;
     const GemmArgs g{a, p.w_bytes > 0 ? packed_w : (const char*)w, lda, (p.w_bytes > 0 ? p.ldk : ws) * 2, (int)rows, (int)k, (int)n * 2, 0, 0, 0, 0};
-    const Out e{dx, k, nullptr, NF_F32, act, q, scale, (int)rows, (int)k, T::code};
+    const Out e{dx, k, nullptr, NF_F32, act, q, scale, (int)rows, (int)k, T::code, nullptr, nullptr, 0};
     if (const int rc = product<T, OUT_GATE, false, true>(g, p.dx, e, slots, s)) return rc;
   }
   if (dw != nullptr) {
@@ -265,8 +312,11 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
     hipLaunchKernelGGL((expand_k<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, q, scale, (int)k, act, (uint16_t*)h, rows);
     if (const int rc = check_launch("expand")) return rc;
     const GemmArgs g{a, h, lda, p.ldk * 2, (int)n, (int)k, (int)rows * 2, 0, 0, 0, 0};
-    const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt};
+    const bool once = p.dw.splits == 1;
+    const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt, p.sums_in_dw ? (float*)sums : nullptr, once ? db : nullptr, db_dt};
     if (const int rc = product<T, OUT_PLAIN, true, true>(g, p.dw, e, slots, s)) return rc;
+    if (p.sums_in_dw && !once)
+      if (const int rc = sum_slots((const float*)sums, p.dw.splits, n, db, db_dt, s)) return rc;
   }
   return 0;
 }

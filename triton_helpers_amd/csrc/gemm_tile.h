@@ -173,10 +173,24 @@ struct Side {
   }
 };
 
+// the sum of a fragment's eight values and s
+template <typename EL>
+__device__ __forceinline__ float add8(i32x4_t v, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int two = v[i];  // (a bit cast of the vector's element itself takes its first one)
+    if constexpr (std::is_same<EL, BF16>::value)
+      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(nf_bf16x2, two), nf_bf16x2{(__bf16)1.0f, (__bf16)1.0f}, s, false);
+    else if constexpr (std::is_same<EL, F16>::value)
+      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(nf_f16x2, two), nf_f16x2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
+  }
+  return s;
+}
+
 template <typename EL, int BM, int BN, int WM, int WN, bool AX = false, bool BX = false>
 struct Gemm {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16, ROWS_M = BM, WAVES_N = WN;
   typedef Side<AX, BM, WAVES> A;
   typedef Side<BX, BN, WAVES> B;
   static constexpr int SLOT = A::BYTES > B::BYTES ? A::BYTES : B::BYTES, SLOTS = 5;
@@ -186,8 +200,9 @@ struct Gemm {
   typedef typename Mma<EL>::acc_t acc_t;
 
   // acc[i][j]: rows m = 16 i + lane % 16 and columns n = 16 j + 4 (lane / 16) + 0..3 of the wave's part
-  template <typename Acc>
-  __device__ static __forceinline__ void run(const GemmArgs& g, const Tile& t, char* lds, Acc (&acc)[FM][FN]) {
+  // SUMS: sums[i] becomes the lane's part of the sum of A's row m (the four lanes with the same lane % 16 hold one each).
+  template <bool SUMS = false, typename Acc>
+  __device__ static __forceinline__ void run(const GemmArgs& g, const Tile& t, char* lds, Acc (&acc)[FM][FN], float* sums = nullptr) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = t.split * g.split_steps;
     const int left = (g.kbytes + STEP - 1) / STEP - first, steps = left < g.split_steps ? left : g.split_steps;
@@ -224,13 +239,14 @@ struct Gemm {
     // One half of a step: its operands are in registers; those of the next half (from the slots at a and b) take their place as they are used up,
     // and `load` sends the loads that fall into this half, one behind each of its first rows of tiles.  (All of them at once, behind the meeting,
     // queue up in front of the matrix instructions.)  The last row's operand moves aside, so that the last read is a row old when the half ends.
-    const auto half = [&](const i32x4_t(&now)[FN], i32x4_t(&then)[FN], const char* a, const char* b, int h, auto&& load, int loads) {
+    const auto half = [&](auto sum_c, const i32x4_t(&now)[FN], i32x4_t(&then)[FN], const char* a, const char* b, int h, auto&& load, int loads) {
       const i32x4_t last = fa[FM - 1];
       fa[FM - 1] = A::read(a, at_a, FM - 1, h);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Mma<EL>::run(now[j], i < FM - 1 ? fa[i] : last, acc[i][j]);
+        if constexpr (decltype(sum_c)::value != 0) sums[i] = add8<EL>(i < FM - 1 ? fa[i] : last, sums[i]);
         if (i < FM - 1) fa[i] = A::read(a, at_a, i, h);
 #pragma unroll
         for (int j = i * FN / (FM - 1); j < (i + 1) * FN / (FM - 1) && j < FN; ++j) then[j] = B::read(b, at_b, j, h);
@@ -247,32 +263,35 @@ struct Gemm {
         // A of the step after the next goes where B of the last step was
         const typename A::Step s = side_a.step((first + step + 2) * STEP, end);
         const uint32_t to = ring + after(slot, 4) * SLOT;
-        half(fb, fc, lds + slot * SLOT, lds + b0 * SLOT, 1, [&](int j) { side_a.load(s, j, to, wave); }, A::LOADS);
+        const auto load = [&](int j) { side_a.load(s, j, to, wave); };
+        half(Int<SUMS>{}, fb, fc, lds + slot * SLOT, lds + b0 * SLOT, 1, load, A::LOADS);
       }
       wait_and_meet<A::LOADS>();
       {
         // B of it where A of this step was
         const typename B::Step s = side_b.step((first + step + 2) * STEP, end);
         const uint32_t to = ring + slot * SLOT;
-        half(fc, fb, lds + a1 * SLOT, lds + b1 * SLOT, 0, [&](int j) { side_b.load(s, j, to, wave); }, B::LOADS);
+        const auto load = [&](int j) { side_b.load(s, j, to, wave); };
+        half(Int<SUMS>{}, fc, fb, lds + a1 * SLOT, lds + b1 * SLOT, 0, load, B::LOADS);
       }
       slot = a1;
     }
     wait_and_meet<0>();  // nothing may still be on its way to LDS when it is used again, or at the workgroup's end
   }
 
-  // The sums in rows: body(m, v) for eight neighbouring columns from column() on, each row of the wave's part once, behind run().  They
+  // The sums in rows: body(m, v, ask(m)) for eight neighbouring columns from column() on, each row of the wave's part once, behind run().  They
   // go through LDS, so that a row leaves in whole cache lines and the code behind them is one short loop (unrolled over the tiles it
-  // costs a small product more in instruction fetches than its sums).
+  // costs a small product more in instruction fetches than its sums).  ask() loads what a row's results go together with: four rows' at once.
   static constexpr int LPR = 2 * FN;  // lanes to a row
   __device__ static __forceinline__ int column(const Tile& t) {
     return t.n * BN + (int)(threadIdx.x >> 6) % WN * (BN / WN) + (int)(threadIdx.x & 63) % LPR * 8;
   }
-  template <typename Acc, typename Body>
-  __device__ static __forceinline__ void each8(const Tile& t, char* lds, const Acc (&acc)[FM][FN], Body&& body) {
+  template <typename Acc, typename Ask, typename Body>
+  __device__ static __forceinline__ void each8(const Tile& t, char* lds, const Acc (&acc)[FM][FN], Ask&& ask, Body&& body) {
     typedef typename std::remove_cv<typename std::remove_reference<decltype(acc[0][0][0])>::type>::type E;
-    constexpr int LD = 16 * FN + 4, PASSES = 16 * FM * LD * 4 * WAVES <= LDS ? 1 : 2, ROWS = 16 * FM / PASSES;
+    constexpr int LD = 16 * FN + 4, PASSES = 16 * FM * LD * 4 * WAVES <= LDS ? 1 : 2, ROWS = 16 * FM / PASSES, STRIDE = 64 / LPR;
     static_assert(ROWS * LD * 4 * WAVES <= LDS, "a strip for every wave");
+    static_assert(ROWS % (4 * STRIDE) == 0, "four rows at a time");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m0 = t.m * BM + wave / WN * (BM / WM);
     E* strip = (E*)lds + wave * (ROWS * LD);
 #pragma unroll
@@ -281,12 +300,20 @@ struct Gemm {
       for (int i = 0; i < FM / PASSES; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) *(Acc*)(strip + (16 * i + (lane & 15)) * LD + 16 * j + 4 * (lane >> 4)) = acc[p * (FM / PASSES) + i][j];
-#pragma unroll 2
-      for (int r = lane / LPR; r < ROWS; r += 64 / LPR) {
-        E v[8];
-        *(Acc*)v = *(const Acc*)(strip + r * LD + lane % LPR * 8);
-        *(Acc*)(v + 4) = *(const Acc*)(strip + r * LD + lane % LPR * 8 + 4);
-        body(m0 + p * ROWS + r, v);
+#pragma unroll 1
+      for (int r = lane / LPR; r < ROWS; r += 4 * STRIDE) {
+        const int m = m0 + p * ROWS + r;
+        decltype(ask(m)) with[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) with[u] = ask(m + u * STRIDE);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          E v[8];
+          const E* from = strip + (r + u * STRIDE) * LD + lane % LPR * 8;
+          *(Acc*)v = *(const Acc*)from;
+          *(Acc*)(v + 4) = *(const Acc*)(from + 4);
+          body(m + u * STRIDE, v, with[u]);
+        }
       }
     }
   }

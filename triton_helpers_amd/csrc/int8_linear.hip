@@ -153,15 +153,15 @@ __global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogu
   if (slots != nullptr) {  // [split][m][n rounded up to 8]
     const int64_t ld = (g.n + 7) / 8 * 8;
     int* o = slots + (int64_t)t.split * g.m * ld + n;
-    G::each8(t, lds, acc, [&](int m, const int (&v)[8]) {
+    G::each8(t, lds, acc, [](int) { return 0; }, [&](int m, const int (&v)[8], int) {
       if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
     });
     return;
   }
   const Columns columns(e, n);
   with_epilogue(e, [&](auto act_c, auto y_c) {
-    G::each8(t, lds, acc, [&](int m, const int (&v)[8]) {
-      if (m < g.m && n < g.n) put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, v, e.s[m], columns);
+    G::each8(t, lds, acc, [&](int m) { return e.s[m < g.m ? m : g.m - 1]; }, [&](int m, const int (&v)[8], float s) {
+      if (m < g.m && n < g.n) put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, v, s, columns);
     });
   });
 }

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_k(Quantize a) {
   __shared__ uint32_t tops[16];
   const int t = threadIdx.x % T;
   const int64_t row = T < 256 ? (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T : blockIdx.x;
-  if (row >= a.rows) return;  // T = 64: whole waves, which meet no barrier
+  if (row >= a.rows) return;  // up to T = 64: all threads of a row, which meet no barrier
   const auto* x = (const typename XT::storage*)a.x + row * a.xs;
   float v[NV][8];
 #pragma unroll
@@ -96,8 +96,12 @@ int quantize_launch(const Quantize& a, hipStream_t s) {
     const int64_t per = T < 256 ? 256 / T : 1;
     hipLaunchKernelGGL((quantize_k<XT, T, NV, ACT, KEEP>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(T < 256 ? 256 : T), 0, s, a);
   };
-  if (a.width <= 512) go(Int<64>{}, Int<1>{});
+  if (a.width <= 128) go(Int<16>{}, Int<1>{});
+  else if (a.width <= 256) go(Int<32>{}, Int<1>{});
+  else if (a.width <= 512) go(Int<64>{}, Int<1>{});
+  else if (a.width <= 1024) go(Int<64>{}, Int<2>{});
   else if (a.width <= 2048) go(Int<64>{}, Int<4>{});
+  else if (a.width <= 4096) go(Int<256>{}, Int<2>{});
   else if (a.width <= 8192) go(Int<256>{}, Int<4>{});
   else if (a.width <= 32768) go(Int<1024>{}, Int<4>{});
   else hipLaunchKernelGGL((quantize_wide_k<XT, ACT, KEEP>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_fwd_k(NormFwd a) {
   __shared__ uint32_t tops[16];
   const int t = threadIdx.x % T;
   const int64_t row = T < 256 ? (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T : blockIdx.x;
-  if (row >= a.rows) return;  // T = 64: whole waves, which meet no barrier
+  if (row >= a.rows) return;  // up to T = 64: all threads of a row, which meet no barrier
   const auto* x = (const typename XT::storage*)a.x + row * a.xs;
   const auto* r = a.r == nullptr ? nullptr : (const typename RT::storage*)a.r + row * a.rs;
   float h[NV][8], w[NV][8];
@@ -316,7 +316,10 @@ int fwd_launch(const NormFwd& a, bool eight, hipStream_t s) {
     hipLaunchKernelGGL((rms_fwd_k<XT, RT, T, NV, E>), dim3((unsigned)blocks), dim3(T < 256 ? 256 : T), 0, s, a);
   };
   const auto by_width = [&](auto e_c) {
-    if (a.width <= 512) go(Int<64>{}, Int<1>{}, e_c);
+    if (a.width <= 128) go(Int<16>{}, Int<1>{}, e_c);
+    else if (a.width <= 256) go(Int<32>{}, Int<1>{}, e_c);
+    else if (a.width <= 512) go(Int<64>{}, Int<1>{}, e_c);
+    else if (a.width <= 1024) go(Int<64>{}, Int<2>{}, e_c);
     else if (a.width <= 2048) go(Int<64>{}, Int<4>{}, e_c);
     else if (a.width <= 4096) go(Int<256>{}, Int<2>{}, e_c);
     else if (a.width <= 8192) go(Int<256>{}, Int<4>{}, e_c);
@@ -336,6 +339,7 @@ int bwd_launch(const NormBwd& a, int64_t groups, hipStream_t s) {
     hipLaunchKernelGGL((rms_bwd_k<XT, HT, T, NV>), dim3((unsigned)((groups + per - 1) / per)), dim3(T < 256 ? 256 : T), 0, s, a);
   };
   if (a.width <= 512) go(Int<64>{}, Int<1>{});
+  else if (a.width <= 1024) go(Int<64>{}, Int<2>{});
   else if (a.width <= 2048) go(Int<64>{}, Int<4>{});
   else if (a.width <= 4096) go(Int<256>{}, Int<2>{});
   else if (a.width <= 8192) go(Int<256>{}, Int<4>{});

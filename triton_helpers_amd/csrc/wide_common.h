@@ -66,15 +66,17 @@ __device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&q)[8]) 
   }
 }
 
-// ---- over the T threads of a row (T = 64: a wave; else the whole workgroup) -----------------
-__device__ __forceinline__ float wave_sum(float v) {
+// ---- over the T threads of a row (up to 64: neighbouring lanes of a wave; else the whole workgroup) -----------------
+template <int T>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  for (int o = T / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+template <int T>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = T / 2; o > 0; o >>= 1) {
     const uint32_t u = __shfl_xor(v, o);
     v = v > u ? v : u;
   }
@@ -83,7 +85,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // `shared`: T / 64 values of its own for every call between two barriers
 template <int T>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
-  v = wave_sum(v);
+  v = lanes_sum<T < 64 ? T : 64>(v);
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -95,7 +97,7 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
 }
 template <int T>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
-  v = wave_max(v);
+  v = lanes_max<T < 64 ? T : 64>(v);
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
