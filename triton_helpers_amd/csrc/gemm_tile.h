@@ -339,7 +339,7 @@ inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit 
 inline bool rows_fit(const void* p, int64_t ld, int64_t bytes) { return bytes % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
 
 // Tiles of 256 x 256, one to a compute unit, or of 128 x 128, two to one (two take 0.57 of the time of a large one, one alone 0.33): what needs
-// less for all of them.  Where even the small ones leave compute units idle the summed dimension is cut into runs of at least four steps.
+// less for all of them.  Where even the small ones leave compute units idle the summed dimension is cut into runs of steps.
 struct TilePlan {
   int bm, splits, split_steps;
   int64_t slot_bytes;
@@ -349,11 +349,17 @@ inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
   TilePlan p{};
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128), last = small % (2 * CUS);
   const double cost_big = (double)((big + CUS - 1) / CUS), cost_small = 0.57 * (double)(small / (2 * CUS)) + (last == 0 ? 0.0 : last <= CUS ? 0.33 : 0.57);
-  p.bm = cost_big <= cost_small ? 256 : 128;
   const int64_t steps = (kbytes + STEP - 1) / STEP;
-  int64_t splits = p.bm == 256 ? 1 : 2 * CUS / small;
-  if (splits > steps / 4) splits = steps / 4;
-  if (splits < 1) splits = 1;
+  p.bm = cost_big <= cost_small ? 256 : 128;
+  int64_t splits = 1;
+  if (p.bm == 128 && small <= CUS) {
+    // us: half a one for a step, and for partial sums another launch, written and read at 4.5 TB/s
+    double best = 0.5 * (double)steps;
+    for (int64_t s = 2; s * small <= 2 * CUS && s * 2 <= steps; s = s < 8 ? s + 1 : s * 5 / 4) {
+      const double cost = 0.5 * (double)((steps + s - 1) / s) + 2.5 + (double)(s * m * n) * 8.0 / 4.5e6;
+      if (cost < best) best = cost, splits = s;
+    }
+  }
   p.split_steps = (int)((steps + splits - 1) / splits);
   p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
   if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 8) * 4, 256);

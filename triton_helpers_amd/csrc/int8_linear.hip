@@ -57,24 +57,30 @@ struct FewRows {
   Epilogue e;
 };
 
-// 16 bytes of a row from any address; bytes beyond the row's end are zeros
+// 16 bytes of a row from any address; bytes beyond the row's end are zeros.  A piece that reaches over the end is read as the row's last 16 bytes
+// and shifted (byte by byte it took longer than all of a short product: 19 x 5000 x 4098 18 us instead of TIME_19).
 __device__ __forceinline__ i32x4_t load16(const char* row, int at, int end) {
-  i32x4_t v = {0, 0, 0, 0};
-  if (at + 16 <= end) {
-    __builtin_memcpy(&v, row + at, 16);
+  uint64_t v[2] = {0, 0};
+  if (end >= 16) {
+    const int from = at < end - 16 ? at : end - 16, gone = at - from;  // bytes that belong in front
+    __builtin_memcpy(v, row + from, 16);
+    const int bits = 8 * (gone & 7);
+    const uint64_t across = bits == 0 ? 0 : v[1] << (64 - bits);
+    const uint64_t lo = v[0] >> bits | across, hi = v[1] >> bits;
+    v[0] = gone < 8 ? lo : gone < 16 ? hi : 0;
+    v[1] = gone < 8 ? hi : 0;
   } else {
-    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 15; ++i)
-      if (at + i < end) w[i / 4] |= (uint32_t)(uint8_t)row[at + i] << (i % 4 * 8);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (int)w[i];
+      if (at + i < end) v[i / 8] |= (uint64_t)(uint8_t)row[at + i] << (i % 8 * 8);
   }
-  return v;
+  i32x4_t r;
+  __builtin_memcpy(&r, v, 16);
+  return r;
 }
 
-// 16 MT rows and 16 NT columns a workgroup.  A wave's unit is 256 bytes of each row, of which the four groups of sixteen lanes take 64 bytes each
-// (whole cache lines of the weights in four loads); the units are dealt to the W waves in turn, and their sums meet in LDS.
+// 16 MT rows and 16 NT columns a workgroup.  A wave's unit is 256 bytes of each row, 64 bytes in each of four loads (the four groups of sixteen
+// lanes take neighbouring pieces); the units are dealt to the W waves in turn, and their sums meet in LDS.
 template <int MT, int NT, int W>
 __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
   __shared__ int part[W][MT * NT][4][64];
@@ -92,33 +98,60 @@ __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
     qp[i] = a.q + (int64_t)(m < a.e.m ? m : a.e.m - 1) * a.ldq;
   }
   i32x4_t acc[MT][NT] = {};
-  const auto unit = [&](int u, auto whole_c) {
-    const int k = u * 256 + g * 64;
-    i32x4_t fw[NT][4], fq[MT][4];
+  struct Unit {
+    i32x4_t w[NT][4], q[MT][4];
+  };
+  const auto load = [&](Unit& f, int u, auto whole_c) {
+    const int k = u * 256 + g * 16;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&fw[j][s], wp[j] + k + 16 * s, 16);
-        else fw[j][s] = load16(wp[j], k + 16 * s, a.k);
+        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&f.w[j][s], wp[j] + k + 64 * s, 16);
+        else f.w[j][s] = load16(wp[j], k + 64 * s, a.k);
       }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&fq[i][s], qp[i] + k + 16 * s, 16);
-        else fq[i][s] = load16(qp[i], k + 16 * s, a.k);
+        if constexpr (decltype(whole_c)::value != 0) __builtin_memcpy(&f.q[i][s], qp[i] + k + 64 * s, 16);
+        else f.q[i][s] = load16(qp[i], k + 64 * s, a.k);
       }
+  };
+  const auto multiply = [&](const Unit& f) {
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<I8>::run(fw[j][s], fq[i][s], acc[i][j]);
+        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<I8>::run(f.w[j][s], f.q[i][s], acc[i][j]);
   };
-  const int whole = a.k / 256;
-  for (int u = wave; u < whole; u += W) unit(u, Int<1>{});
-  if (whole * 256 < a.k && whole % W == wave) unit(whole, Int<0>{});
+  // (the scales and biases of the results that this thread will write are asked for before anything else)
+  static_assert(MT * NT * 32 <= 64 * W, "a thread for every eight results");
+  const int ej = threadIdx.x % (2 * NT), em = threadIdx.x / (2 * NT), en = n0 + 8 * ej;  // columns 8 j.. of row m
+  const bool writes = em < 16 * MT && em < a.e.m && en < a.e.n;
+  const Columns columns(a.e, writes ? en : a.e.n);
+  const float es = writes ? a.e.s[em] : 0.0f;
+  const int units = (a.k + 255) / 256;
+  const auto load_any = [&](Unit& f, int u) {
+    if ((u + 1) * 256 <= a.k) load(f, u, Int<1>{});
+    else load(f, u, Int<0>{});
+  };
+  int u = wave;
+  if constexpr (MT * NT <= 2) {  // two units' loads at once
+    for (; u + W < units; u += 2 * W) {
+      Unit f, h;
+      load(f, u, Int<1>{});
+      load_any(h, u + W);
+      multiply(f);
+      multiply(h);
+    }
+  }
+  for (; u < units; u += W) {
+    Unit f;
+    load_any(f, u);
+    multiply(f);
+  }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -127,19 +160,14 @@ __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
       for (int c = 0; c < 4; ++c) part[wave][i * NT + j][c][lane] = acc[i][j][c];
   __syncthreads();
   // a thread adds up eight neighbouring columns of a row: lane and numbers as the matrix instruction left them
-  for (int at = threadIdx.x; at < MT * NT * 32; at += 64 * W) {
-    const int j = at % (2 * NT), m = at / (2 * NT), n = n0 + 8 * j;  // columns 8 j.. of row m
-    if (m >= a.e.m || n >= a.e.n) continue;
-    const Columns columns(a.e, n);
-    const float s = a.e.s[m];
-    const int from = (j & 1) * 32 + (m & 15), tile = (m >> 4) * NT + (j >> 1);
-    int sum[8] = {};
+  if (!writes) return;
+  const int from = (ej & 1) * 32 + (em & 15), tile = (em >> 4) * NT + (ej >> 1);
+  int sum[8] = {};
 #pragma unroll
-    for (int v = 0; v < W; ++v)
+  for (int v = 0; v < W; ++v)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) sum[c] += part[v][tile][c & 3][from + (c >> 2) * 16];
-    with_epilogue(a.e, [&](auto act_c, auto y_c) { put8<decltype(act_c)::value, decltype(y_c)>(a.e, m, n, sum, s, columns); });
-  }
+    for (int c = 0; c < 8; ++c) sum[c] += part[v][tile][c & 3][from + (c >> 2) * 16];
+  with_epilogue(a.e, [&](auto act_c, auto y_c) { put8<decltype(act_c)::value, decltype(y_c)>(a.e, em, en, sum, es, columns); });
 }
 
 // ---- tiles --------------------------------------------------------------------------------------
@@ -258,9 +286,24 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
       constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
       hipLaunchKernelGGL((int8_few_rows_k<MT, NT, 8>), dim3((unsigned)((n + 16 * NT - 1) / (16 * NT))), dim3(512), 0, s, a);
     };
-    if (rows <= 16) go(Int<1>{}, Int<1>{});
-    else if (rows <= 32) go(Int<2>{}, Int<1>{});
-    else go(Int<4>{}, Int<2>{});
+    // More columns to a workgroup read the rows less often, but leave compute units idle: the least of what the busiest unit loads.  us with 1, 2, 4 groups
+    // of 16 columns: 16 rows x 4096 x 16384 18.9, 17.3, 16.5, x 4096 6.8, 8.1, 12.0; 64 rows 42.8, 31.6, 25.5 and 12.1, 14.2, 21.3;
+    // 32 x 5000 x 4098 13.9, 11.0, 16.6.  (Sixteen waves instead of eight: never faster, up to 1.5 times slower.)
+    const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    int nt = 1;
+    int64_t least = INT64_MAX;
+    for (int t = 1; t <= (rows <= 4 ? 1 : 4); t *= 2) {
+      const int64_t blocks = (n + 16 * t - 1) / (16 * t), load = (blocks + 255) / 256 * (t + mt);
+      if (load < least) least = load, nt = t;
+    }
+    const auto by_columns = [&](auto mt_c) {
+      if (nt == 1) go(mt_c, Int<1>{});
+      else if (nt == 2) go(mt_c, Int<2>{});
+      else go(mt_c, Int<4>{});
+    };
+    if (mt == 1) by_columns(Int<1>{});
+    else if (mt == 2) by_columns(Int<2>{});
+    else by_columns(Int<4>{});
     return check_launch("int8_linear");
   }
   char* ws = (char*)workspace;

@@ -96,7 +96,10 @@ int quantize_launch(const Quantize& a, hipStream_t s) {
     const int64_t per = T < 256 ? 256 / T : 1;
     hipLaunchKernelGGL((quantize_k<XT, T, NV, ACT, KEEP>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(T < 256 ? 256 : T), 0, s, a);
   };
-  if (a.width <= 128) go(Int<16>{}, Int<1>{});
+  // a few rows: as many threads to each as its values take
+  if (a.rows <= 512 && a.width > 512 && a.width <= 2048) go(Int<256>{}, Int<1>{});
+  else if (a.rows <= 256 && a.width > 2048 && a.width <= 8192) go(Int<1024>{}, Int<1>{});
+  else if (a.width <= 128) go(Int<16>{}, Int<1>{});
   else if (a.width <= 256) go(Int<32>{}, Int<1>{});
   else if (a.width <= 512) go(Int<64>{}, Int<1>{});
   else if (a.width <= 1024) go(Int<64>{}, Int<2>{});

@@ -177,8 +177,10 @@ struct NormBwd {
 template <typename XT, typename HT, int T, int NV>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_bwd_k(NormBwd a) {
   __shared__ float sums[2][16];
+  constexpr int PER = T < 256 ? 256 / T : 1;  // groups of a workgroup
+  __shared__ float others[PER > 1 ? PER - 1 : 1][PER > 1 ? T * NV * 8 : 1];
   const int t = threadIdx.x % T;
-  const int64_t per = T < 256 ? 256 / T : 1, groups = gridDim.x * per, group = blockIdx.x * per + threadIdx.x / T;
+  const int64_t groups = (int64_t)gridDim.x * PER, group = blockIdx.x * PER + threadIdx.x / T;
   float dw[NV][8] = {}, w[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -219,12 +221,27 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_bwd_k(NormBwd a) {
       if (a.dr != nullptr) store8<HT>((typename HT::storage*)a.dr + row * a.width + c, a.width - c, d);
     }
   }
-  if (a.slots != nullptr) {
+  if (a.slots == nullptr) return;
+  if constexpr (PER > 1) {  // the workgroup's groups leave one slot
+    if (threadIdx.x >= T) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * T + t) * 8;
-      store8<F32>(a.slots + group * a.width + c, a.width - c, dw[j]);
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) others[threadIdx.x / T - 1][(j * 8 + i) * T + t] = dw[j][i];
     }
+    __syncthreads();
+    if (threadIdx.x >= T) return;
+#pragma unroll
+    for (int k = 0; k < PER - 1; ++k)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[j][i] += others[k][(j * 8 + i) * T + t];
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * T + t) * 8;
+    store8<F32>(a.slots + (int64_t)blockIdx.x * a.width + c, a.width - c, dw[j]);
   }
 }
 
@@ -277,34 +294,33 @@ __global__ __launch_bounds__(1024) void rms_bwd_wide_k(NormBwd a) {
 
 // column sums of the groups' partial sums, in a fixed order (the same bits on every run)
 __global__ __launch_bounds__(1024) void sum_slots_k(const float* slots, int64_t groups, int width, void* out, int dt) {
-  __shared__ float part[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+  __shared__ float part[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
   float s = 0.0f;
   if (c < width) {
 #pragma unroll 8
-    for (int64_t k = g; k < groups; k += 16) s += slots[k * width + c];
+    for (int64_t k = g; k < groups; k += 32) s += slots[k * width + c];
   }
-  part[g][threadIdx.x & 63] = s;
+  part[g][threadIdx.x & 31] = s;
   __syncthreads();
   if (g == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
+    for (int i = 1; i < 32; ++i) s += part[i][threadIdx.x];
     store_any(out, c, dt, s);
   }
 }
-
 int sum_slots(const float* slots, int64_t groups, int64_t width, void* out, int dt, hipStream_t s) {
-  hipLaunchKernelGGL(sum_slots_k, dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, s, slots, groups, (int)width, out, dt);
+  hipLaunchKernelGGL(sum_slots_k, dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, s, slots, groups, (int)width, out, dt);
   return check_launch("sum_slots");
 }
 
 constexpr int NORM_ONE_PASS = 32768;  // the widest row that a workgroup's registers hold
 // Threads that share a row.  (A wave's row needs no barrier; a workgroup's asks for a row with more loads at once.)
 inline int norm_threads(int width) { return width <= 2048 ? 64 : width <= 8192 ? 256 : 1024; }
-// Groups of a backward: each walks several rows and leaves one row of partial sums of dw.
+// Groups of a backward: each walks as many rows as the others, and a workgroup of them leaves one row of partial sums of dw.
 inline int64_t norm_groups(int64_t rows, int width) {
-  const int64_t most = width <= 2048 ? 4096 : width <= 8192 ? 1024 : 256;
-  return rows < most ? rows : most;
+  const int64_t most = width <= 2048 ? 4096 : width <= 8192 ? 1024 : 256, each = (rows + most - 1) / most;
+  return (rows + each - 1) / each;
 }
 
 template <typename XT, typename RT>
@@ -316,7 +332,10 @@ int fwd_launch(const NormFwd& a, bool eight, hipStream_t s) {
     hipLaunchKernelGGL((rms_fwd_k<XT, RT, T, NV, E>), dim3((unsigned)blocks), dim3(T < 256 ? 256 : T), 0, s, a);
   };
   const auto by_width = [&](auto e_c) {
-    if (a.width <= 128) go(Int<16>{}, Int<1>{}, e_c);
+    // a few rows: as many threads to each as its values take, for the time of one row is that of its loads and sums
+    if (a.rows <= 512 && a.width > 512 && a.width <= 2048) go(Int<256>{}, Int<1>{}, e_c);
+    else if (a.rows <= 256 && a.width > 2048 && a.width <= 8192) go(Int<1024>{}, Int<1>{}, e_c);
+    else if (a.width <= 128) go(Int<16>{}, Int<1>{}, e_c);
     else if (a.width <= 256) go(Int<32>{}, Int<1>{}, e_c);
     else if (a.width <= 512) go(Int<64>{}, Int<1>{}, e_c);
     else if (a.width <= 1024) go(Int<64>{}, Int<2>{}, e_c);
@@ -348,10 +367,10 @@ int bwd_launch(const NormBwd& a, int64_t groups, hipStream_t s) {
   return check_launch("rms_norm_bwd");
 }
 
-// the slots that the launch writes: whole workgroups of them
+// the slots that the launch writes: one for each workgroup
 inline int64_t slot_rows(int64_t rows, int width) {
   const int64_t g = norm_groups(rows, width);
-  return norm_threads(width) == 64 ? (g + 3) / 4 * 4 : g;
+  return norm_threads(width) == 64 ? (g + 3) / 4 : g;
 }
 
 }  // namespace nf
