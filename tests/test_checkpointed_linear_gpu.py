@@ -85,8 +85,53 @@ def test_large(m, n, k, dtype, name):
 
 
 @pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m", [16383, 16384, 16385, 16415, 40001])
+@pytest.mark.parametrize("n,k", [(8, 8), (64, 128), (128, 64), (136, 120), (120, 136), (256, 256), (248, 32), (16, 256), (128, 128), (264, 256), (256, 264)])
+def test_many_rows_few_channels(m, n, k, dtype):
+    """Around the sizes from which, and up to which, a workgroup keeps the layer's weights."""
+    args = whole(m, n, k, dtype, seed=m + n, bias=k != 64)
+    check_exact(step(*args, "relu"), exact(*args, "relu"))
+
+
+def test_many_rows_parts():
+    """Strided rows and weights, absent gradients, nothing kept, float32 gradients, where a workgroup keeps the weights."""
+    m, n, k = 20011, 64, 72
+    x, w, b, dy = whole(m, n, k, torch.bfloat16)
+    want = exact(x, w, b, dy, "relu")
+    wide = [torch.full((t.shape[0], t.shape[1] + 24), 99.0, device=DEV, dtype=t.dtype) for t in (x, w, dy)]
+    for at in (8, 3):  # on and off 16-byte boundaries
+        views = [v[:, at : at + t.shape[1]] for v, t in zip(wide, (x, w, dy))]
+        for v, t in zip(views, (x, w, dy)):
+            v.copy_(t)
+        check_exact(step(views[0], views[1], b, views[2], "relu"), want)
+        check_exact(step(views[0], w, b, dy, "relu"), want)
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1)):
+        leaves = [t.clone().requires_grad_(bool(r)) for t, r in zip((x, w, b), need)]
+        checkpointed_linear(*leaves, "relu").backward(dy)
+        for t, r, g in zip(leaves, need, want[1:]):
+            assert (t.grad is not None) == bool(r) and (not r or torch.equal(t.grad, g))
+    with torch.no_grad():
+        assert torch.equal(checkpointed_linear(x, w, b, "relu"), want[0])
+        assert torch.equal(checkpointed_linear(x, w), (x.double() @ w.double().t()).bfloat16())
+    bl, wl = b.float().requires_grad_(), w.float().requires_grad_()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = checkpointed_linear(x, wl, bl, "relu")
+    y.backward(dy)
+    assert torch.equal(wl.grad.double(), dy.double().t() @ x.double().clamp_min(0)) and torch.equal(bl.grad.double(), dy.double().sum(0))
+    # rows without an 8-bit form
+    x[7, 3], x[m - 1, 0] = float("nan"), -float("inf")
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = checkpointed_linear(xl, wl, b, "gelu")
+    y.backward(dy)
+    keep = torch.ones(m, dtype=torch.bool, device=DEV)
+    keep[7] = keep[m - 1] = False
+    assert torch.isnan(y[7]).all() and torch.isfinite(y[keep]).all() and torch.isnan(wl.grad).all()
+    assert torch.isnan(xl.grad[~keep]).all() and torch.isfinite(xl.grad[keep]).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("name", ["none", "relu", "relu2", "silu", "gelu"])
-@pytest.mark.parametrize("m,n,k", [(1, 70, 90), (300, 70, 90), (300, 136, 2500), (5000, 64, 48)])
+@pytest.mark.parametrize("m,n,k", [(1, 70, 90), (300, 70, 90), (300, 136, 2500), (5000, 64, 48), (17000, 64, 48), (17000, 200, 256)])
 def test_activations(m, n, k, dtype, name):
     g = torch.Generator(device=DEV).manual_seed(k)
     x, w, b, dy = ((torch.randn(*s, generator=g, device=DEV) * c).to(dtype) for s, c in (((m, k), 2), ((n, k), k**-0.5), ((n,), 1), ((m, n), 1)))

@@ -6,6 +6,7 @@
 // Three products of 2 M N K operations on the 16-bit matrix instructions (gemm_tile.h).  The forward's lie along the summed dimension; dx takes W,
 // and dW both dy and act(x^), crosswise, as they are in memory.  The gate of dx is applied to the sums in registers.  act(x) and act(x^) are
 // written out in 16 bits by streams of their own (a product reads its operand once for each 256 channels of the result).
+#include "checkpointed_narrow.h"
 #include "gemm_tile.h"
 
 namespace nf {
@@ -24,14 +25,6 @@ struct Out {
   void* db;     // ... or, of a single run, where they go, in type db_dt
   int db_dt;
 };
-
-// v * act'(x^); a closed gate lets nothing through, not even an infinity
-template <int ACT>
-__device__ __forceinline__ float gated(float v, float x) {
-  if constexpr (ACT == NF_ACT_NONE) return v;
-  else if constexpr (ACT == NF_ACT_RELU || ACT == NF_ACT_RELU2) return x <= 0.0f ? 0.0f : v * act_slope<ACT>(x);
-  else return v * act_slope<ACT>(x);
-}
 
 // the gate of eight columns of a row
 struct Gate {
@@ -212,6 +205,7 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
   else go(Int<256>{}, Int<4>{}, Int<2>{});
   const int rc = check_launch("checkpointed_linear");
   if (rc != 0 || p.splits == 1) return rc;
+  if (MODE == OUT_PLAIN && e.n % 8 == 0 && (int64_t)e.m * e.n < (1ll << 31)) return sum_slots(slots, p.splits, (int64_t)e.m * e.n, e.y, e.y_dt, s);
   hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 7) / 8) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
   return check_launch("checkpointed_linear_sum");
 }
@@ -221,6 +215,7 @@ inline bool sizes_ok(int64_t rows, int64_t n, int64_t k) {
 }
 
 struct KeepFwd {
+  bool narrow;
   int64_t ldh, h_bytes, w_bytes;
   TilePlan tile;
   int64_t total() const { return h_bytes + w_bytes + tile.slot_bytes; }
@@ -228,6 +223,8 @@ struct KeepFwd {
 KeepFwd keep_fwd(const void* x, int64_t xs, const void* w, int64_t ws, int64_t rows, int64_t n, int64_t k, int act) {
   KeepFwd p{};
   p.ldh = round_up(k, 8);
+  p.narrow = narrow_fits(rows, n, k) && rows_fit(x, xs * 2, k * 2) && rows_fit(w, ws * 2, k * 2);
+  if (p.narrow) return p;
   if (act != NF_ACT_NONE || !rows_fit(x, xs * 2, k * 2)) p.h_bytes = round_up(rows * p.ldh * 2, 256);
   if (!rows_fit(w, ws * 2, k * 2)) p.w_bytes = round_up(n * p.ldh * 2, 256);
   p.tile = tile_plan(rows, n, k * 2);
@@ -235,6 +232,7 @@ KeepFwd keep_fwd(const void* x, int64_t xs, const void* w, int64_t ws, int64_t r
 }
 
 struct KeepBwd {
+  bool narrow;
   int64_t ldk, ldn, dy_bytes, w_bytes, h_bytes, sum_bytes;
   int strips, groups;
   bool sums_in_dw;
@@ -246,6 +244,12 @@ KeepBwd keep_bwd(const void* dy, int64_t dys, const void* w, int64_t ws, int64_t
   KeepBwd p{};
   p.ldk = round_up(k, 8);
   p.ldn = round_up(n, 8);
+  p.narrow = need_dw && narrow_fits(rows, n, k) && rows_fit(dy, dys * 2, n * 2) && (!need_dx || rows_fit(w, ws * 2, k * 2));
+  if (p.narrow) {
+    p.groups = narrow_groups(rows);
+    p.sum_bytes = round_up((int64_t)p.groups * n * 4, 256) + (int64_t)p.groups * n * k * 4;
+    return p;
+  }
   if ((need_dx || need_dw) && !rows_fit(dy, dys * 2, n * 2)) p.dy_bytes = round_up(rows * p.ldn * 2, 256);
   if (need_dx) {
     if (!rows_fit(w, ws * 2, k * 2)) p.w_bytes = round_up(n * p.ldk * 2, 256);
@@ -273,6 +277,7 @@ int fwd(const KeepFwd& p, const void* x, int64_t xs, const void* w, int64_t ws, 
   char *h = at, *packed = at + p.h_bytes;
   float* slots = (float*)(packed + p.w_bytes);
   hipStream_t s = (hipStream_t)stream;
+  if (p.narrow) return narrow_fwd({x, w, bias, y, q, scale, xs, ws, ys, rows, (int)n, (int)k, bias_dt, act}, T::code, s);
   if (q != nullptr || p.h_bytes > 0)
     if (const int rc = nf_quantize_rows(x, xs, T::code, q, scale, p.h_bytes > 0 ? h : nullptr, p.ldh, act, rows, k, stream)) return rc;
   if (p.w_bytes > 0)
@@ -288,6 +293,13 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
         void* db, int db_dt, int64_t rows, int64_t n, int64_t k, int act, char* at, hipStream_t s) {
   char *packed_dy = at, *packed_w = packed_dy + p.dy_bytes, *h = packed_w + p.w_bytes, *sums = h + p.h_bytes;
   float* slots = (float*)(sums + p.sum_bytes);
+  if (p.narrow) {
+    float *part_db = (float*)sums, *part_dw = (float*)(sums + round_up((int64_t)p.groups * n * 4, 256));
+    if (const int rc = narrow_bwd({dy, w, q, scale, dx, part_dw, db == nullptr ? nullptr : part_db, dys, ws, rows, (int)n, (int)k, act}, T::code, s)) return rc;
+    if (db != nullptr)
+      if (const int rc = sum_slots(part_db, p.groups, n, db, db_dt, s)) return rc;
+    return sum_slots(part_dw, p.groups, n * k, dw, dw_dt, s);
+  }
   if (db != nullptr && !p.sums_in_dw) {
     hipLaunchKernelGGL((column_sums_k<T>), dim3(p.strips, p.groups), dim3(256), 0, s, (const uint16_t*)dy, dys, rows, (int)n, (float*)sums);
     if (const int rc = check_launch("column_sums")) return rc;

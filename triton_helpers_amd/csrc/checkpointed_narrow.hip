@@ -1,0 +1,334 @@
+// The linear layer with 8-bit checkpoints where rows are many and channels few (both sides at most 256): streams over the rows.
+//
+//   forward   a row is read once: its largest magnitude, its 8-bit form out, act(x) in 16 bits to LDS, the product with weights that sit in the
+//             waves' registers, y out
+//   backward  dy and q are read once: act(x^) to LDS, dW's sums (256 x 256 in the eight waves' registers for as long as the workgroup lives), dx with
+//             weights that sit in LDS, its gate, dx out; the workgroups' dW and db are added up afterwards, in a fixed order
+//
+// As separate passes (8-bit rows; act(x^); three products) the same bytes move two and a half times.  2^18 x 256 x 256 with ReLU, forward and backward:
+// NARROW_STEP.
+//
+// A workgroup of 512 threads takes 32 rows at a time.  Rows in LDS lie as in Side's crosswise form (gemm_tile.h): the 32-byte segments of a row are
+// spread by its bits 0, 1 and 3, free of bank conflicts for the transposing reads and for 16-byte reads along the row alike.
+#include "checkpointed_narrow.h"
+#include "gemm_tile.h"
+
+namespace nf {
+
+constexpr int TILE = 32, THREADS = 512;
+
+// 16 bytes, piece p of a row of 2 C bytes
+template <int C>
+__device__ __forceinline__ int place(int row, int p) {
+  const int spread = (row & 3) | (row >> 1 & 4);
+  return row * (2 * C) + (((p >> 1) ^ spread) << 5 | (p & 1) << 4);
+}
+// the sixteen rows from `row` on, along the row: piece 4 step + lane / 16
+template <int C>
+__device__ __forceinline__ i32x4_t along(const char* from, int row, int step, int lane) {
+  return *(const i32x4_t*)(from + place<C>(row + (lane & 15), 4 * step + (lane >> 4)));
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(i32x4_t v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (uint32_t)v[i];
+    f[2 * i] = T::to_f32((uint16_t)w);
+    f[2 * i + 1] = T::to_f32((uint16_t)(w >> 16));
+  }
+}
+template <typename T>
+__device__ __forceinline__ i32x4_t pack8(const float (&f)[8]) {
+  i32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (int)T::pack(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+__device__ __forceinline__ i32x4_t load_piece(const uint16_t* p, bool there) {
+  i32x4_t v = {0, 0, 0, 0};
+  if (there) v = *(const i32x4_t*)p;
+  return v;
+}
+
+// ---- forward ------------------------------------------------------------------------------------
+template <typename T, int KP, int NP>
+__global__ __launch_bounds__(THREADS, 2) void narrow_fwd_k(NarrowFwd a) {
+  constexpr int PIECES = KP / 8, ROWS = THREADS / PIECES, EACH = TILE / ROWS;  // threads to a row, rows at once, rows of a thread
+  constexpr int NT = NP / 128, STEPS = KP / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[2][TILE * KP * 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+  const int p = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES;
+  const bool in = p * 8 < a.k;
+  // the weights of this wave's columns, and their biases
+  i32x4_t w[NT][STEPS];
+  float b[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = wave * (16 * NT) + 16 * j;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int c = 32 * s + 8 * g;
+      w[j][s] = load_piece((const uint16_t*)a.w + (int64_t)(n + i16) * a.ws + c, n + i16 < a.n && c < a.k);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[j][i] = a.bias != nullptr && n + 4 * g + i < a.n ? load_as_f32(a.bias, n + 4 * g + i, a.bias_dt) : 0.0f;
+  }
+  const int64_t tiles = (a.rows + TILE - 1) / TILE;
+  i32x4_t x[EACH];
+  const auto ask = [&](int64_t tile) {
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int64_t row = tile * TILE + r0 + j * ROWS;
+      x[j] = load_piece((const uint16_t*)a.x + row * a.xs + p * 8, in && row < a.rows);
+    }
+  };
+  ask(blockIdx.x);
+  int turn = 0;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int r = r0 + j * ROWS;
+      const int64_t row = tile * TILE + r;
+      float v[8];
+      unpack8<T>(x[j], v);
+      if (a.q != nullptr) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t m = magnitude_bits(v[i]);
+          top = top > m ? top : m;
+        }
+        const EightBit e = eight_bit(lanes_max<PIECES>(top));
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = quantized(v[i], e);
+        if (row < a.rows) {
+          if (in) store8_q(a.q + row * a.k + p * 8, 8, q);
+          if (p == 0) a.scale[row] = e.scale;
+        }
+      }
+      if (a.act != NF_ACT_NONE) {
+        with_act(a.act, [&](auto act_c) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(act_c)::value>(v[i]);
+        });
+        x[j] = pack8<T>(v);
+      }
+      *(i32x4_t*)(lds[turn] + place<KP>(r, p)) = x[j];
+    }
+    __syncthreads();  // (the other buffer's readers met here in the last round)
+    ask(tile + gridDim.x);
+    f32x4_t acc[2][NT] = {};
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const i32x4_t f = along<KP>(lds[turn], 16 * i, s, lane);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::run(w[j][s], f, acc[i][j]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = tile * TILE + 16 * i + i16;
+      if (row >= a.rows) continue;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int n = wave * (16 * NT) + 16 * j + 4 * g;
+        const uint32_t o[2] = {T::pack(acc[i][j][0] + b[j][0], acc[i][j][1] + b[j][1]), T::pack(acc[i][j][2] + b[j][2], acc[i][j][3] + b[j][3])};
+        if (n < a.n) __builtin_memcpy((uint16_t*)a.y + row * a.ys + n, o, 8);  // n: a multiple of 8 channels
+      }
+    }
+  }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+template <typename T, int KP, int NP>
+__global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
+  constexpr int PD = NP / 8, RD = THREADS / PD, ED = TILE / RD;  // dy: threads to a row, rows at once, rows of a thread
+  constexpr int PQ = KP / 8, RQ = THREADS / PQ, EQ = TILE / RQ;  // q
+  constexpr int XT = KP / 128, STEPS = NP / 32;                  // dx: tiles of 16 columns of a wave; steps of the sum
+  constexpr int WN = NP / 64, WK = KP / 32;                      // dW: tiles of a wave, four waves along n and two along k
+  typedef Side<true, NP, 8> D;
+  typedef Side<true, KP, 8> H;
+  __shared__ __attribute__((aligned(1024))) char lds[NP * KP * 2 + TILE * NP * 2 + TILE * KP * 2];
+  char *wl = lds, *dl = lds + NP * KP * 2, *hl = dl + TILE * NP * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
+  const int pd = threadIdx.x % PD, rd = threadIdx.x / PD, pq = threadIdx.x % PQ, rq = threadIdx.x / PQ;
+  const bool want_x = a.dx != nullptr;
+  if (want_x) {
+    for (int r = rq; r < NP; r += RQ)
+      *(i32x4_t*)(wl + place<KP>(r, pq)) = load_piece((const uint16_t*)a.w + (int64_t)r * a.ws + pq * 8, r < a.n && pq * 8 < a.k);
+  }
+  const int64_t tiles = (a.rows + TILE - 1) / TILE;
+  i32x4_t d[ED];
+  int q[EQ][2];
+  float s[EQ];
+  const auto ask = [&](int64_t tile) {
+#pragma unroll
+    for (int j = 0; j < ED; ++j) {
+      const int64_t row = tile * TILE + rd + j * RD;
+      d[j] = load_piece((const uint16_t*)a.dy + row * a.dys + pd * 8, row < a.rows && pd * 8 < a.n);
+    }
+#pragma unroll
+    for (int j = 0; j < EQ; ++j) {
+      const int64_t row = tile * TILE + rq + j * RQ;
+      q[j][0] = q[j][1] = 0;
+      s[j] = 0.0f;
+      if (row < a.rows && pq * 8 < a.k) {
+        __builtin_memcpy(q[j], a.q + row * a.k + pq * 8, 8);
+        s[j] = a.scale[row];
+      }
+    }
+  };
+  ask(blockIdx.x);
+  f32x4_t aw[WN][WK] = {};
+  float sums[8] = {};
+  const int wn = wave >> 1, wk = wave & 1;
+  const int at_d = D::read_at(lane, wn * WN), at_h = H::read_at(lane, wk * WK), at_w = H::read_at(lane, wave * XT);
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+#pragma unroll
+    for (int j = 0; j < ED; ++j) {
+      *(i32x4_t*)(dl + place<NP>(rd + j * RD, pd)) = d[j];
+      if (a.db != nullptr) {
+        float v[8];
+        unpack8<T>(d[j], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[i] += v[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < EQ; ++j) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = s[j] * (float)(q[j][i / 4] << (24 - i % 4 * 8) >> 24);
+      with_act(a.act, [&](auto act_c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(act_c)::value>(v[i]);
+      });
+      *(i32x4_t*)(hl + place<KP>(rq + j * RQ, pq)) = pack8<T>(v);
+    }
+    __syncthreads();
+    // the gate of this wave's results (the rows were read a round ago), and the next round's rows
+    int gq[2][XT];
+    float gs[2];
+    if (want_x && a.act != NF_ACT_NONE) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t row = tile * TILE + 16 * i + i16;
+        gs[i] = row < a.rows ? a.scale[row] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < XT; ++j) {
+          const int c = wave * (16 * XT) + 16 * j + 4 * g;
+          gq[i][j] = 0;
+          if (row < a.rows && c < a.k) __builtin_memcpy(&gq[i][j], a.q + row * a.k + c, 4);
+        }
+      }
+    }
+    ask(tile + gridDim.x);
+    {
+      i32x4_t fd[WN];
+#pragma unroll
+      for (int i = 0; i < WN; ++i) fd[i] = D::read(dl, at_d, i, 0);
+#pragma unroll
+      for (int j = 0; j < WK; ++j) {
+        const i32x4_t f = H::read(hl, at_h, j, 0);
+#pragma unroll
+        for (int i = 0; i < WN; ++i) aw[i][j] = Mma<T>::run(f, fd[i], aw[i][j]);
+      }
+    }
+    if (want_x) {
+      f32x4_t ax[2][XT] = {};
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t) {
+        i32x4_t f[XT];
+#pragma unroll
+        for (int j = 0; j < XT; ++j) f[j] = H::read(wl, at_w, j, t);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const i32x4_t r = along<NP>(dl, 16 * i, t, lane);
+#pragma unroll
+          for (int j = 0; j < XT; ++j) ax[i][j] = Mma<T>::run(f[j], r, ax[i][j]);
+        }
+      }
+      with_act(a.act, [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t row = tile * TILE + 16 * i + i16;
+#pragma unroll
+          for (int j = 0; j < XT; ++j) {
+            const int c = wave * (16 * XT) + 16 * j + 4 * g;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[e] = ax[i][j][e];
+              if constexpr (ACT != NF_ACT_NONE) v[e] = gated<ACT>(v[e], gs[i] * (float)(gq[i][j] << (24 - e * 8) >> 24));
+            }
+            const uint32_t o[2] = {T::pack(v[0], v[1]), T::pack(v[2], v[3])};
+            if (row < a.rows && c < a.k) __builtin_memcpy((uint16_t*)a.dx + row * a.k + c, o, 8);
+          }
+        }
+      });
+    }
+    __syncthreads();  // the tiles have been read
+  }
+  float* dw = a.dw + (int64_t)blockIdx.x * a.n * a.k;
+#pragma unroll
+  for (int i = 0; i < WN; ++i)
+#pragma unroll
+    for (int j = 0; j < WK; ++j) {
+      const int n = (wn * WN + i) * 16 + i16, c = (wk * WK + j) * 16 + 4 * g;
+      if (n < a.n && c < a.k) *(f32x4_t*)(dw + (int64_t)n * a.k + c) = aw[i][j];
+    }
+  if (a.db != nullptr) {  // RD threads hold parts of the same columns
+    float* part = (float*)lds;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[rd * NP + pd * 8 + i] = sums[i];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < a.n) {
+      float v = part[c];
+      for (int r = 1; r < RD; ++r) v += part[r * NP + c];
+      a.db[(int64_t)blockIdx.x * a.n + c] = v;
+    }
+  }
+}
+
+constexpr int NARROW = 256, NARROW_MIN_ROWS = 16384, NARROW_GROUPS = 256;
+
+bool narrow_fits(int64_t rows, int64_t n, int64_t k) { return rows >= NARROW_MIN_ROWS && n <= NARROW && k <= NARROW && n % 8 == 0 && k % 8 == 0; }
+int narrow_groups(int64_t rows) {
+  const int64_t tiles = (rows + TILE - 1) / TILE;
+  return (int)(tiles < NARROW_GROUPS ? tiles : NARROW_GROUPS);
+}
+
+template <typename Body>
+void by_size(int k, int n, Body&& body) {
+  if (k <= 128 && n <= 128) body(Int<128>{}, Int<128>{});
+  else if (k <= 128) body(Int<128>{}, Int<256>{});
+  else if (n <= 128) body(Int<256>{}, Int<128>{});
+  else body(Int<256>{}, Int<256>{});
+}
+
+int narrow_fwd(const NarrowFwd& a, int dtype, hipStream_t s) {
+  const int64_t tiles = (a.rows + TILE - 1) / TILE;
+  const unsigned blocks = (unsigned)(tiles < 512 ? tiles : 512);  // two to a compute unit
+  by_size(a.k, a.n, [&](auto k_c, auto n_c) {
+    constexpr int KP = decltype(k_c)::value, NP = decltype(n_c)::value;
+    if (dtype == NF_F16) hipLaunchKernelGGL((narrow_fwd_k<F16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((narrow_fwd_k<BF16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
+  });
+  return check_launch("checkpointed_narrow_fwd");
+}
+
+int narrow_bwd(const NarrowBwd& a, int dtype, hipStream_t s) {
+  const unsigned blocks = (unsigned)narrow_groups(a.rows);
+  by_size(a.k, a.n, [&](auto k_c, auto n_c) {
+    constexpr int KP = decltype(k_c)::value, NP = decltype(n_c)::value;
+    if (dtype == NF_F16) hipLaunchKernelGGL((narrow_bwd_k<F16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((narrow_bwd_k<BF16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
+  });
+  return check_launch("checkpointed_narrow_bwd");
+}
+
+}  // namespace nf

@@ -281,7 +281,8 @@ struct Gemm {
 
   // The sums in rows: body(m, v, ask(m)) for eight neighbouring columns from column() on, each row of the wave's part once, behind run().  They
   // go through LDS, so that a row leaves in whole cache lines and the code behind them is one short loop (unrolled over the tiles it
-  // costs a small product more in instruction fetches than its sums).  ask() loads what a row's results go together with: four rows' at once.
+  // costs a small product more in instruction fetches than its sums).  ask() loads what a row's results go together with: for all rows of a pass at
+  // once, ahead of the pass before.
   static constexpr int LPR = 2 * FN;  // lanes to a row
   __device__ static __forceinline__ int column(const Tile& t) {
     return t.n * BN + (int)(threadIdx.x >> 6) % WN * (BN / WN) + (int)(threadIdx.x & 63) % LPR * 8;
@@ -291,29 +292,30 @@ struct Gemm {
     typedef typename std::remove_cv<typename std::remove_reference<decltype(acc[0][0][0])>::type>::type E;
     constexpr int LD = 16 * FN + 4, PASSES = 16 * FM * LD * 4 * WAVES <= LDS ? 1 : 2, ROWS = 16 * FM / PASSES, STRIDE = 64 / LPR;
     static_assert(ROWS * LD * 4 * WAVES <= LDS, "a strip for every wave");
-    static_assert(ROWS % (4 * STRIDE) == 0, "four rows at a time");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m0 = t.m * BM + wave / WN * (BM / WM);
     E* strip = (E*)lds + wave * (ROWS * LD);
+    constexpr int N = ROWS / STRIDE;  // rows of a lane and pass
+    decltype(ask(0)) with[2][N];
+    const auto ask_all = [&](int p) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) with[p & 1][u] = ask(m0 + p * ROWS + lane / LPR + u * STRIDE);
+    };
+    ask_all(0);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
 #pragma unroll
       for (int i = 0; i < FM / PASSES; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) *(Acc*)(strip + (16 * i + (lane & 15)) * LD + 16 * j + 4 * (lane >> 4)) = acc[p * (FM / PASSES) + i][j];
-#pragma unroll 1
-      for (int r = lane / LPR; r < ROWS; r += 4 * STRIDE) {
-        const int m = m0 + p * ROWS + r;
-        decltype(ask(m)) with[4];
+      if (p + 1 < PASSES) ask_all(p + 1);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) with[u] = ask(m + u * STRIDE);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          E v[8];
-          const E* from = strip + (r + u * STRIDE) * LD + lane % LPR * 8;
-          *(Acc*)v = *(const Acc*)from;
-          *(Acc*)(v + 4) = *(const Acc*)(from + 4);
-          body(m + u * STRIDE, v, with[u]);
-        }
+      for (int u = 0; u < N; ++u) {
+        const int r = lane / LPR + u * STRIDE;
+        E v[8];
+        const E* from = strip + r * LD + lane % LPR * 8;
+        *(Acc*)v = *(const Acc*)from;
+        *(Acc*)(v + 4) = *(const Acc*)(from + 4);
+        body(m0 + p * ROWS + r, v, with[p & 1][u]);
       }
     }
   }
@@ -353,10 +355,11 @@ inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
   p.bm = cost_big <= cost_small ? 256 : 128;
   int64_t splits = 1;
   if (p.bm == 128 && small <= CUS) {
-    // us: half a one for a step, and for partial sums another launch, written and read at 4.5 TB/s
-    double best = 0.5 * (double)steps;
-    for (int64_t s = 2; s * small <= 2 * CUS && s * 2 <= steps; s = s < 8 ? s + 1 : s * 5 / 4) {
-      const double cost = 0.5 * (double)((steps + s - 1) / s) + 2.5 + (double)(s * m * n) * 8.0 / 4.5e6;
+    // us: 0.85 for a step (what memory takes to answer; 2^18 rows into 256 x 256 took 142 instead of 62 with 27 runs instead of 128), and for
+    // partial sums another launch, written and read at 4.5 TB/s
+    double best = 1e30;
+    for (int64_t s = 1; s == 1 || (s * small <= 2 * CUS && s * 2 <= steps); s = s < 8 ? s + 1 : s * 5 / 4) {
+      const double cost = 0.85 * (double)((steps + s - 1) / s) + (s == 1 ? 0.0 : 2.5 + (double)(s * m * n) * 8.0 / 4.5e6);
       if (cost < best) best = cost, splits = s;
     }
   }

@@ -150,6 +150,14 @@ __device__ __forceinline__ float act_slope(float z) {
     return cdf + z * pdf;
   } else return 1.0f;
 }
+// v * act'(x^); a closed gate lets nothing through, not even an infinity
+template <int ACT>
+__device__ __forceinline__ float gated(float v, float x) {
+  if constexpr (ACT == NF_ACT_NONE) return v;
+  else if constexpr (ACT == NF_ACT_RELU || ACT == NF_ACT_RELU2) return x <= 0.0f ? 0.0f : v * act_slope<ACT>(x);
+  else return v * act_slope<ACT>(x);
+}
+
 template <int V>
 using Int = std::integral_constant<int, V>;
 
