@@ -49,6 +49,18 @@ __device__ __forceinline__ i32x4_t load_piece(const uint16_t* p, bool there) {
   if (there) v = *(const i32x4_t*)p;
   return v;
 }
+// The rows of a tile as a buffer: loads outside of it give zeros and stores do nothing, without a branch (behind branches the compiler cannot count
+// what is under way, and waits for all of it).
+constexpr int NOWHERE = -16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* p, int64_t row, int64_t rows, int64_t ld, int bytes) {
+  const int64_t left = rows - row;
+  const int have = left < 0 ? 0 : left < TILE ? (int)left : TILE;
+  const int size = have == 0 ? 0 : (have - 1) * (int)ld + bytes;
+  return __builtin_amdgcn_make_buffer_rsrc((char*)p + (have == 0 ? 0 : row * ld), 0, size, 0x00020000);
+}
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ i32x4_t get16(__amdgpu_buffer_rsrc_t b, int at) { return __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0)); }
 
 // ---- forward ------------------------------------------------------------------------------------
 template <typename T, int KP, int NP>
@@ -74,70 +86,90 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_fwd_k(NarrowFwd a) {
     for (int i = 0; i < 4; ++i) b[j][i] = a.bias != nullptr && n + 4 * g + i < a.n ? load_as_f32(a.bias, n + 4 * g + i, a.bias_dt) : 0.0f;
   }
   const int64_t tiles = (a.rows + TILE - 1) / TILE;
-  i32x4_t x[EACH];
-  const auto ask = [&](int64_t tile) {
+  const auto ask = [&](int64_t tile, i32x4_t(&x)[EACH]) {
+    const auto buffer = rows_of(a.x, tile * TILE, a.rows, a.xs * 2, a.k * 2);
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int64_t row = tile * TILE + r0 + j * ROWS;
-      x[j] = load_piece((const uint16_t*)a.x + row * a.xs + p * 8, in && row < a.rows);
-    }
+    for (int j = 0; j < EACH; ++j) x[j] = get16(buffer, in ? (r0 + j * ROWS) * (int)a.xs * 2 + p * 16 : NOWHERE);
   };
-  ask(blockIdx.x);
-  int turn = 0;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+  const auto prepare = [&](int64_t tile, i32x4_t(&x)[EACH], char* to) {
+    float v[EACH][8];
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int r = r0 + j * ROWS;
-      const int64_t row = tile * TILE + r;
-      float v[8];
-      unpack8<T>(x[j], v);
-      if (a.q != nullptr) {
-        uint32_t top = 0;
+    for (int j = 0; j < EACH; ++j) unpack8<T>(x[j], v[j]);
+    if (a.q != nullptr) {
+      const auto to_q = rows_of(a.q, tile * TILE, a.rows, a.k, a.k);
+      const auto to_s = rows_of(a.scale, tile * TILE, a.rows, 4, 4);
+      uint32_t top[EACH];
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        top[j] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t m = magnitude_bits(v[i]);
-          top = top > m ? top : m;
-        }
-        const EightBit e = eight_bit(lanes_max<PIECES>(top));
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = quantized(v[i], e);
-        if (row < a.rows) {
-          if (in) store8_q(a.q + row * a.k + p * 8, 8, q);
-          if (p == 0) a.scale[row] = e.scale;
+          const uint32_t m = magnitude_bits(v[j][i]);
+          top[j] = top[j] > m ? top[j] : m;
         }
       }
-      if (a.act != NF_ACT_NONE) {
-        with_act(a.act, [&](auto act_c) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(act_c)::value>(v[i]);
-        });
-        x[j] = pack8<T>(v);
+      for (int j = 0; j < EACH; ++j) top[j] = lanes_max<PIECES>(top[j]);
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int r = r0 + j * ROWS;
+        const EightBit e = eight_bit(top[j]);
+        u32x2_t q = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i / 4] |= ((uint32_t)(int)quantized(v[j][i], e) & 255u) << (i % 4 * 8);
+        __builtin_amdgcn_raw_buffer_store_b64(q, to_q, in ? r * a.k + p * 8 : NOWHERE, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(e.scale), to_s, p == 0 ? r * 4 : NOWHERE, 0, 0);
       }
-      *(i32x4_t*)(lds[turn] + place<KP>(r, p)) = x[j];
     }
-    __syncthreads();  // (the other buffer's readers met here in the last round)
-    ask(tile + gridDim.x);
+    if (a.act != NF_ACT_NONE) {
+      with_act(a.act, [&](auto act_c) {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[j][i] = act_value<decltype(act_c)::value>(v[j][i]);
+      });
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) x[j] = pack8<T>(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) *(i32x4_t*)(to + place<KP>(r0 + j * ROWS, p)) = x[j];
+  };
+  // between two meetings a wave multiplies one tile and prepares the next, so that one wave's vector arithmetic runs beside another's products;
+  // the rows of two more tiles are under way
+  const int64_t far = gridDim.x;
+  const auto round = [&](int64_t tile, const char* from, char* to, i32x4_t(&x)[EACH]) {
     f32x4_t acc[2][NT] = {};
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const i32x4_t f = along<KP>(lds[turn], 16 * i, s, lane);
+        const i32x4_t f = along<KP>(from, 16 * i, s, lane);
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::run(w[j][s], f, acc[i][j]);
       }
+    const auto to_y = rows_of(a.y, tile * TILE, a.rows, a.ys * 2, a.n * 2);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int64_t row = tile * TILE + 16 * i + i16;
-      if (row >= a.rows) continue;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int n = wave * (16 * NT) + 16 * j + 4 * g;
-        const uint32_t o[2] = {T::pack(acc[i][j][0] + b[j][0], acc[i][j][1] + b[j][1]), T::pack(acc[i][j][2] + b[j][2], acc[i][j][3] + b[j][3])};
-        if (n < a.n) __builtin_memcpy((uint16_t*)a.y + row * a.ys + n, o, 8);  // n: a multiple of 8 channels
+        const int n = wave * (16 * NT) + 16 * j + 4 * g;  // (n: a multiple of 8 channels)
+        const u32x2_t o = {T::pack(acc[i][j][0] + b[j][0], acc[i][j][1] + b[j][1]), T::pack(acc[i][j][2] + b[j][2], acc[i][j][3] + b[j][3])};
+        __builtin_amdgcn_raw_buffer_store_b64(o, to_y, n < a.n ? (16 * i + i16) * (int)a.ys * 2 + n * 2 : NOWHERE, 0, 0);
       }
-    }
+    __builtin_amdgcn_sched_barrier(0);  // the wait for the next tile's rows stays behind the products
+    prepare(tile + far, x, to);
+    ask(tile + 3 * far, x);
+    __syncthreads();
+  };
+  i32x4_t x0[EACH], x1[EACH];
+  ask(blockIdx.x, x0);
+  ask(blockIdx.x + far, x1);
+  prepare(blockIdx.x, x0, lds[0]);
+  ask(blockIdx.x + 2 * far, x0);
+  __syncthreads();
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += 2 * far) {
+    round(tile, lds[0], lds[1], x1);
+    round(tile + far, lds[1], lds[0], x0);
   }
 }
 
@@ -164,20 +196,16 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
   int q[EQ][2];
   float s[EQ];
   const auto ask = [&](int64_t tile) {
+    const auto from_d = rows_of(a.dy, tile * TILE, a.rows, a.dys * 2, a.n * 2), from_q = rows_of(a.q, tile * TILE, a.rows, a.k, a.k),
+               from_s = rows_of(a.scale, tile * TILE, a.rows, 4, 4);
 #pragma unroll
-    for (int j = 0; j < ED; ++j) {
-      const int64_t row = tile * TILE + rd + j * RD;
-      d[j] = load_piece((const uint16_t*)a.dy + row * a.dys + pd * 8, row < a.rows && pd * 8 < a.n);
-    }
+    for (int j = 0; j < ED; ++j) d[j] = get16(from_d, pd * 8 < a.n ? (rd + j * RD) * (int)a.dys * 2 + pd * 16 : NOWHERE);
 #pragma unroll
     for (int j = 0; j < EQ; ++j) {
-      const int64_t row = tile * TILE + rq + j * RQ;
-      q[j][0] = q[j][1] = 0;
-      s[j] = 0.0f;
-      if (row < a.rows && pq * 8 < a.k) {
-        __builtin_memcpy(q[j], a.q + row * a.k + pq * 8, 8);
-        s[j] = a.scale[row];
-      }
+      const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(from_q, pq * 8 < a.k ? (rq + j * RQ) * a.k + pq * 8 : NOWHERE, 0, 0);
+      q[j][0] = (int)v[0];
+      q[j][1] = (int)v[1];
+      s[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from_s, (rq + j * RQ) * 4, 0, 0));
     }
   };
   ask(blockIdx.x);
@@ -212,15 +240,14 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
     int gq[2][XT];
     float gs[2];
     if (want_x && a.act != NF_ACT_NONE) {
+      const auto from_q = rows_of(a.q, tile * TILE, a.rows, a.k, a.k), from_s = rows_of(a.scale, tile * TILE, a.rows, 4, 4);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int64_t row = tile * TILE + 16 * i + i16;
-        gs[i] = row < a.rows ? a.scale[row] : 0.0f;
+        gs[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from_s, (16 * i + i16) * 4, 0, 0));
 #pragma unroll
         for (int j = 0; j < XT; ++j) {
           const int c = wave * (16 * XT) + 16 * j + 4 * g;
-          gq[i][j] = 0;
-          if (row < a.rows && c < a.k) __builtin_memcpy(&gq[i][j], a.q + row * a.k + c, 4);
+          gq[i][j] = (int)__builtin_amdgcn_raw_buffer_load_b32(from_q, c < a.k ? (16 * i + i16) * a.k + c : NOWHERE, 0, 0);
         }
       }
     }
@@ -252,9 +279,9 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
       }
       with_act(a.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
+        const auto to_x = rows_of(a.dx, tile * TILE, a.rows, (int64_t)a.k * 2, a.k * 2);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int64_t row = tile * TILE + 16 * i + i16;
 #pragma unroll
           for (int j = 0; j < XT; ++j) {
             const int c = wave * (16 * XT) + 16 * j + 4 * g;
@@ -264,8 +291,7 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
               v[e] = ax[i][j][e];
               if constexpr (ACT != NF_ACT_NONE) v[e] = gated<ACT>(v[e], gs[i] * (float)(gq[i][j] << (24 - e * 8) >> 24));
             }
-            const uint32_t o[2] = {T::pack(v[0], v[1]), T::pack(v[2], v[3])};
-            if (row < a.rows && c < a.k) __builtin_memcpy((uint16_t*)a.dx + row * a.k + c, o, 8);
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{T::pack(v[0], v[1]), T::pack(v[2], v[3])}, to_x, c < a.k ? (16 * i + i16) * a.k * 2 + c * 2 : NOWHERE, 0, 0);
           }
         }
       });
@@ -312,9 +338,10 @@ void by_size(int k, int n, Body&& body) {
 
 int narrow_fwd(const NarrowFwd& a, int dtype, hipStream_t s) {
   const int64_t tiles = (a.rows + TILE - 1) / TILE;
-  const unsigned blocks = (unsigned)(tiles < 512 ? tiles : 512);  // two to a compute unit
   by_size(a.k, a.n, [&](auto k_c, auto n_c) {
     constexpr int KP = decltype(k_c)::value, NP = decltype(n_c)::value;
+    constexpr int64_t most = KP == 256 && NP == 256 ? 256 : 512;  // one workgroup to a compute unit, of the smaller ones two
+    const unsigned blocks = (unsigned)(tiles < most ? tiles : most);
     if (dtype == NF_F16) hipLaunchKernelGGL((narrow_fwd_k<F16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
     else hipLaunchKernelGGL((narrow_fwd_k<BF16, KP, NP>), dim3(blocks), dim3(THREADS), 0, s, a);
   });

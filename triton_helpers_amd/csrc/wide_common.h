@@ -67,20 +67,36 @@ __device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&q)[8]) 
 }
 
 // ---- over the T threads of a row (up to 64: neighbouring lanes of a wave; else the whole workgroup) -----------------
-template <int T>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = T / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// (lane exchanges inside the vector unit: through LDS each costs some hundred clocks, one behind the other)
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int T, typename V, typename Join>
+__device__ __forceinline__ V lanes_join(V v, Join&& join) {
+  const auto bits = [](V x) { return __builtin_bit_cast(uint32_t, x); };
+  const auto value = [](uint32_t x) { return __builtin_bit_cast(V, x); };
+  if constexpr (T >= 2) v = join(v, value(moved<0xb1>(bits(v))));    // neighbours in pairs
+  if constexpr (T >= 4) v = join(v, value(moved<0x4e>(bits(v))));    // pairs in fours
+  if constexpr (T >= 8) v = join(v, value(moved<0x141>(bits(v))));   // mirrored eights
+  if constexpr (T >= 16) v = join(v, value(moved<0x140>(bits(v))));  // mirrored sixteens
+  if constexpr (T >= 32) {  // odd sixteens against even ones
+    const auto w = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    v = join(value(w[0]), value(w[1]));
+  }
+  if constexpr (T >= 64) {
+    const auto w = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = join(value(w[0]), value(w[1]));
+  }
   return v;
 }
 template <int T>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_join<T>(v, [](float x, float y) { return x + y; });
+}
+template <int T>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-#pragma unroll
-  for (int o = T / 2; o > 0; o >>= 1) {
-    const uint32_t u = __shfl_xor(v, o);
-    v = v > u ? v : u;
-  }
-  return v;
+  return lanes_join<T>(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
 }
 // `shared`: T / 64 values of its own for every call between two barriers
 template <int T>
