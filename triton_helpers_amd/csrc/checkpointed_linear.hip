@@ -138,26 +138,58 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
   });
 }
 
-// act(s q) in 16 bits, rows filled up with zeros to whole 16-byte pieces; a stream, eight values a thread
+// What the backward's products read and the caller does not have: copies of dy and W on 16-byte boundaries, and act(s q) in 16 bits, each with rows
+// filled up with zeros to whole 16-byte pieces.  A stream, 16 bytes a thread; one launch for all of them (of what a small layer's step takes,
+// launches are the most).
+struct Copy {
+  const char* from;
+  int64_t ld, rows;
+  char* to;
+  int bytes;
+  int64_t blocks;  // none: nothing to copy
+};
+struct Prepare {
+  Copy copy[2];
+  const int8_t* q;
+  const float* s;
+  uint16_t* h;
+  int64_t rows;
+  int width, act;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void expand_k(const int8_t* q, const float* s, int width, int act, uint16_t* h, int64_t rows) {
-  const int pieces = (width + 7) / 8;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= rows * pieces) return;
+__global__ __launch_bounds__(256) void prepare_k(Prepare a) {
+  int64_t block = blockIdx.x;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (block < a.copy[c].blocks) {
+      const Copy& m = a.copy[c];
+      const int pieces = (m.bytes + 15) / 16;
+      const int64_t at = block * 256 + threadIdx.x;
+      if (at >= m.rows * pieces) return;
+      const int64_t row = at / pieces;
+      const int k = (int)(at - row * pieces) * 16;
+      *(i32x4_t*)(m.to + at * 16) = load16(m.from + row * m.ld, k, m.bytes);
+      return;
+    }
+    block -= a.copy[c].blocks;
+  }
+  const int pieces = (a.width + 7) / 8;
+  const int64_t at = block * 256 + threadIdx.x;
+  if (at >= a.rows * pieces) return;
   const int64_t row = at / pieces;
-  const int c = (int)(at - row * pieces) * 8, n = width - c;
-  const int8_t* p = q + row * width + c;
+  const int c = (int)(at - row * pieces) * 8, n = a.width - c;
+  const int8_t* p = a.q + row * a.width + c;
   int8_t raw[8];
   if (n >= 8) __builtin_memcpy(raw, p, 8);
   else
 #pragma unroll
     for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (int8_t)0;
-  const float scale = s[row];
-  with_act(act, [&](auto act_c) {
+  const float scale = a.s[row];
+  with_act(a.act, [&](auto act_c) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? act_value<decltype(act_c)::value>(scale * (float)raw[i]) : 0.0f;
-    store8<T>(h + at * 8, 8, v);
+    store8<T>(a.h + at * 8, 8, v);
   });
 }
 
@@ -305,24 +337,30 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
     if (const int rc = check_launch("column_sums")) return rc;
     if (const int rc = sum_slots((const float*)sums, p.groups, n, db, db_dt, s)) return rc;
   }
-  const char* a = (const char*)dy;
-  int64_t lda = dys * 2;
-  if (p.dy_bytes > 0) {
-    if (const int rc = pack_rows(a, lda, n * 2, packed_dy, rows, s)) return rc;
-    a = packed_dy;
-    lda = p.ldn * 2;
+  Prepare make{};
+  int64_t blocks = 0;
+  const auto copy = [&](int i, const void* from, int64_t ld, int64_t count, int64_t width, char* to) {
+    make.copy[i] = {(const char*)from, ld * 2, count, to, (int)width * 2, (count * ((width + 7) / 8) + 255) / 256};
+    blocks += make.copy[i].blocks;
+  };
+  if (p.dy_bytes > 0) copy(0, dy, dys, rows, n, packed_dy);
+  if (p.w_bytes > 0) copy(1, w, ws, n, k, packed_w);
+  if (dw != nullptr) {
+    make.q = q, make.s = scale, make.h = (uint16_t*)h, make.rows = rows, make.width = (int)k, make.act = act;
+    blocks += (rows * (p.ldk / 8) + 255) / 256;
   }
+  if (blocks > 0) {
+    hipLaunchKernelGGL((prepare_k<T>), dim3((unsigned)blocks), dim3(256), 0, s, make);
+    if (const int rc = check_launch("checkpointed_linear_prepare")) return rc;
+  }
+  const char* a = p.dy_bytes > 0 ? packed_dy : (const char*)dy;
+  const int64_t lda = (p.dy_bytes > 0 ? p.ldn : dys) * 2;
   if (dx != nullptr) {
-    if (p.w_bytes > 0)
-      if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed_w, n, s)) return rc;
     const GemmArgs g{a, p.w_bytes > 0 ? packed_w : (const char*)w, lda, (p.w_bytes > 0 ? p.ldk : ws) * 2, (int)rows, (int)k, (int)n * 2, 0, 0, 0, 0};
     const Out e{dx, k, nullptr, NF_F32, act, q, scale, (int)rows, (int)k, T::code, nullptr, nullptr, 0};
     if (const int rc = product<T, OUT_GATE, false, true>(g, p.dx, e, slots, s)) return rc;
   }
   if (dw != nullptr) {
-    const int64_t pieces = rows * (p.ldk / 8);
-    hipLaunchKernelGGL((expand_k<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, q, scale, (int)k, act, (uint16_t*)h, rows);
-    if (const int rc = check_launch("expand")) return rc;
     const GemmArgs g{a, h, lda, p.ldk * 2, (int)n, (int)k, (int)rows * 2, 0, 0, 0, 0};
     const bool once = p.dw.splits == 1;
     const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt, p.sums_in_dw ? (float*)sums : nullptr, once ? db : nullptr, db_dt};

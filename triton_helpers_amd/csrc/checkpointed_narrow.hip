@@ -320,9 +320,13 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
   }
 }
 
-constexpr int NARROW = 256, NARROW_MIN_ROWS = 16384, NARROW_GROUPS = 256;
+constexpr int NARROW = 256, NARROW_GROUPS = 256;
 
-bool narrow_fits(int64_t rows, int64_t n, int64_t k) { return rows >= NARROW_MIN_ROWS && n <= NARROW && k <= NARROW && n % 8 == 0 && k % 8 == 0; }
+// From how many rows on these kernels are the quicker ones (forward + backward, us, here / as separate passes, GELU): 64 x 64 2048 rows 20 / 35, 128 x 128
+// 23 / 36, 64 x 256 25 / 37; 256 x 256 2048 rows 47 / 43, 8192 56 / 52, 16384 59 / 65, 2^18 231 / 353 (ReLU).
+bool narrow_fits(int64_t rows, int64_t n, int64_t k) {
+  return n <= NARROW && k <= NARROW && n % 8 == 0 && k % 8 == 0 && rows >= (n > 128 && k > 128 ? 12288 : 2048);
+}
 int narrow_groups(int64_t rows) {
   const int64_t tiles = (rows + TILE - 1) / TILE;
   return (int)(tiles < NARROW_GROUPS ? tiles : NARROW_GROUPS);
