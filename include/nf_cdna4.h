@@ -315,7 +315,7 @@ int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int8_t* q, fl
                      int64_t width, void* stream);
 
 /* y[m, n] = act(scale[m] * w_scale[n] * sum_k q[m, k] * w[n, k] + bias[n]) for int8 q [rows, k] and w [n, k] (row strides in values, at least k), exact
- * 32-bit integer sums (k at most 131071), float32 behind them, rounded once to y's type.  bias: NULL or [n] of any type.  Up to 64 rows
+ * 32-bit integer sums (k at most 131071, n at most 2^26), float32 behind them, rounded once to y's type.  bias: NULL or [n] of any type.  Up to 64 rows
  * need no workspace; nf_int8_linear_workspace_bytes() says what the call with these pointers and strides needs, 16-byte aligned (copies of
  * rows off 16-byte boundaries, partial sums where the summed dimension is split). */
 int64_t nf_int8_linear_workspace_bytes(const int8_t* q, int64_t q_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k);
@@ -327,7 +327,7 @@ int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const 
  *   forward   y[m, n] = sum_k act(x[m, k]) w[n, k] + bias[n];  q, scale: the 8-bit rows of x (NULL both: nothing is kept)
  *   backward  x^ = scale q;  dx = (dy w) * act'(x^);  dw = dy^T act(x^);  db = column sums of dy; each written, each may be NULL
  * Sums in float32; act(x) and act(x^) enter the products rounded to the rows' type.  bias and db of any type, dw of the rows' type or float32.  dx and
- * q [rows, k] and dw [n, k] without gaps.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and
+ * q [rows, k] and dw [n, k] without gaps; y, q and dx on 16-byte boundaries, y's rows too where n is a multiple of 8.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and
  * strides).  Results are the same bits on every run.  The backward wants at least one row; w may be NULL without dx, q and scale where
  * neither dw nor an activation's dx needs them. */
 int64_t nf_linear_keep_fwd_workspace_bytes(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k, int act);

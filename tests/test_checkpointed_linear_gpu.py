@@ -239,6 +239,17 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(db, sum(dy[i : i + 2**17].double().sum(0) for i in range(0, m, 2**17)).to(torch.bfloat16))
 
 
+def test_more_pieces_than_one_row_of_a_grid():
+    """act(x^) and a copied dy of more than 2^28 pieces of 16 bytes; only the last rows have gradients."""
+    m, n, k, tail = 2**21 + 3, 12, 1030, 45
+    x, w, b, dy = whole(m, n, k, torch.bfloat16)
+    dy[:-tail] = 0
+    got = step(x, w, b, dy, "relu")
+    want = exact(x[-tail:], w, b, dy[-tail:], "relu")
+    check_exact([got[0][-tail:], got[1][-tail:], *got[2:]], want)
+    assert got[1][:-tail].abs().max() == 0
+
+
 def test_rows_that_are_not_finite():
     """They are NaN where they are used, and nothing else is."""
     for name in ("none", "relu", "gelu"):

@@ -173,6 +173,13 @@ def test_quantize_rows(width, dtype):
     assert all(torch.equal(a, b) for a, b in zip(quantize_rows(wide[:, 5 : 5 + width]), quantize_rows(wide[:, 5 : 5 + width].contiguous())))
 
 
+def test_quantize_more_rows_than_one_launch_takes():
+    x = torch.randn(2**21 + 9, 8, device=DEV)
+    q, s = quantize_rows(x)
+    for part in (slice(0, 50), slice(2**21 - 20, x.shape[0])):
+        assert all(torch.equal(a, b) for a, b in zip(quantize_rows(x[part]), (q[part], s[part])))
+
+
 def test_another_stream_and_captured():
     q, s, w, t, b = case(200, 264, 8192, torch.float32)
     few = q[:3].contiguous()

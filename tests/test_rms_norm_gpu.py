@@ -216,6 +216,29 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(a, b) and torch.equal(xl.grad, cl.grad)
 
 
+def test_more_rows_than_one_launch_takes():
+    rows = 2**21 + 37
+    x = torch.randn(rows, 8, device=DEV, dtype=torch.bfloat16)
+    r = torch.randn(rows, 8, device=DEV)
+    w = torch.randn(8, device=DEV)
+    y, s = rms_norm(x, w, EPS, r)
+    q, scale, s8 = rms_norm_int8(x, w, EPS, r)
+    check_forward(y, s, x, r, w)
+    assert torch.equal(s8, s)
+    for part in (slice(0, 50), slice(2**21 - 20, rows)):
+        alone = rms_norm_int8(x[part], w, EPS, r[part])
+        assert torch.equal(alone[0], q[part]) and torch.equal(alone[1], scale[part])
+
+
+def test_the_residual_is_the_input():
+    x, _, w, dy, ds = inputs(20, 100, torch.float32, torch.float32, torch.float32)
+    xl = x.clone().requires_grad_()
+    y, s = rms_norm(xl, w, EPS, xl)
+    torch.autograd.backward((y, s), (dy, ds))
+    full = step(x, x.clone(), w, dy, ds)
+    assert torch.equal(y, full[0]) and torch.equal(s, full[1]) and torch.equal(xl.grad, full[2] + full[3])
+
+
 def test_no_rows_and_absent_gradients():
     w = torch.ones(64, device=DEV, requires_grad=True)
     x = torch.empty(0, 64, device=DEV, requires_grad=True)

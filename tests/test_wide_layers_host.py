@@ -27,7 +27,7 @@ def test_norm_entry_points():
     refused(fwd(rows=-1), -1, b"rows")
     refused(fwd(rows=2**31), -1, b"rows")
     refused(fwd(width=0), -1, b"width")
-    refused(fwd(width=2**30 + 1), -1, b"width")
+    refused(fwd(width=2**26 + 1), -1, b"width")
     refused(fwd(eps=ctypes.c_float(-1.0)), -1, b"eps")
     refused(fwd(x=None), -1, b"NULL")
     refused(fwd(xs=63), -1, b"stride")
@@ -86,6 +86,8 @@ def test_product_entry_points():
     refused(product(rows=-1), -1, b"rows")
     refused(product(n=0), -1, b"n=0")
     refused(product(k=0), -1, b"k=0")
+    refused(product(n=2**26 + 1, ys=2**27), -1, b"n=")
+    refused(product(rows=2**31 - 1, n=2**20, ys=2**20, work=16, size=2**62), -2, b"more tiles")
     refused(product(k=131072, qs=131072, ws=131072), -2, b"131071")
     refused(product(s=None), -1, b"NULL")
     refused(product(qs=63), -1, b"stride")
@@ -149,7 +151,7 @@ def test_keep_entry_points():
     refused(fwd(dt=F32), -2, b"float16 or bfloat16")
     refused(fwd(bdt=5), -1, b"dtype")
     refused(fwd(act=7), -1, b"activation")
-    for bad in ({"rows": 2**30}, {"rows": -1}, {"n": 0}, {"k": 0}, {"k": 2**29}):
+    for bad in ({"rows": 2**30}, {"rows": -1}, {"n": 0}, {"k": 0}, {"k": 2**26 + 1}, {"n": 2**26 + 1}):
         refused(fwd(**bad), -1, b"rows")
     refused(fwd(w=None), -1, b"NULL")
     refused(fwd(s=None), -1, b"NULL")
@@ -182,6 +184,15 @@ def test_keep_entry_points():
     refused(bwd(work=16, size=need - 1), -1, b"workspace")
     refused(bwd(work=8, size=need), -1, b"workspace")
     assert bwd(dx=None, dw=None, db=None) == 0
+    # where a workgroup keeps the weights the results want whole pieces
+    refused(fwd(rows=4096, y=24), -3, b"boundaries")
+    refused(fwd(rows=4096, q=24), -3, b"boundaries")
+    refused(fwd(rows=4096, ys=52), -3, b"boundaries")
+    big = lib.nf_linear_keep_bwd_workspace_bytes(16, 48, 16, 64, 4096, 48, 64, 1, 1, 1)
+    assert big >= 128 * 48 * (64 + 1) * 4
+    refused(bwd(rows=4096, dx=24, work=16, size=big), -3, b"boundaries")
+    refused(bwd(rows=4096, work=16, size=big - 1), -1, b"workspace")
+    refused(bwd(rows=2**29, k=2**20, ws=2**20, n=264, ds=264, work=16, size=2**62), -2, b"more tiles")
 
 
 def test_keep_arguments():

@@ -158,7 +158,7 @@ struct Prepare {
 };
 template <typename T>
 __global__ __launch_bounds__(256) void prepare_k(Prepare a) {
-  int64_t block = blockIdx.x;
+  int64_t block = block_number();
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (block < a.copy[c].blocks) {
@@ -243,7 +243,7 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
 }
 
 inline bool sizes_ok(int64_t rows, int64_t n, int64_t k) {
-  return rows > 0 && rows < (1ll << 30) && n >= 1 && n < (1ll << 29) && k >= 1 && k < (1ll << 29);
+  return rows > 0 && rows <= (1ll << 29) && n >= 1 && n <= MOST_WIDTH && k >= 1 && k <= MOST_WIDTH;
 }
 
 struct KeepFwd {
@@ -350,7 +350,7 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
     blocks += (rows * (p.ldk / 8) + 255) / 256;
   }
   if (blocks > 0) {
-    hipLaunchKernelGGL((prepare_k<T>), dim3((unsigned)blocks), dim3(256), 0, s, make);
+    hipLaunchKernelGGL((prepare_k<T>), grid_of(blocks), dim3(256), 0, s, make);
     if (const int rc = check_launch("checkpointed_linear_prepare")) return rc;
   }
   const char* a = p.dy_bytes > 0 ? packed_dy : (const char*)dy;
@@ -387,10 +387,13 @@ extern "C" int nf_linear_keep_fwd(const void* x, int64_t x_stride, int dtype, co
   NF_REQUIRE(dtype_ok(bias_dtype), NF_EINVAL, "unknown dtype code %d", bias_dtype);
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
   if (rows == 0) return 0;
-  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows below 2^30, channels 1..2^29-1", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows up to 2^29, channels 1..2^26", (long long)rows, (long long)n, (long long)k);
   NF_REQUIRE(x && w && y && (q == nullptr) == (scale == nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE((rows == 1 || (x_stride >= k && y_stride >= n)) && (n == 1 || w_stride >= k), NF_EINVAL, "row stride below the row's length");
   const KeepFwd p = keep_fwd(x, x_stride, w, w_stride, rows, n, k, act);
+  NF_REQUIRE(p.narrow || tiles_fit(p.tile, rows, n), NF_EUNSUPPORTED, "rows=%lld, n=%lld: more tiles than a launch holds", (long long)rows, (long long)n);
+  NF_REQUIRE(!p.narrow || ((uintptr_t)y % 16 == 0 && y_stride % 8 == 0 && y_stride < (1 << 21) && (uintptr_t)q % 16 == 0 && (uintptr_t)scale % 4 == 0), NF_EALIGN,
+             "y, its rows and q want 16-byte boundaries");
   NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
              "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
   return dtype == NF_F16 ? fwd<F16>(p, x, x_stride, w, w_stride, bias, bias_dtype, y, y_stride, q, scale, rows, n, k, act, (char*)workspace, stream)
@@ -408,13 +411,16 @@ extern "C" int nf_linear_keep_bwd(const void* dy, int64_t dy_stride, int dtype, 
   NF_REQUIRE(dtype == NF_F16 || dtype == NF_BF16, NF_EUNSUPPORTED, "dtype code %d: float16 or bfloat16 rows", dtype);
   NF_REQUIRE((dw_dtype == dtype || dw_dtype == NF_F32) && dtype_ok(db_dtype), NF_EUNSUPPORTED, "the weight's gradient is of the rows' type or float32");
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
-  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows 1..2^30-1, channels 1..2^29-1", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows 1..2^29, channels 1..2^26", (long long)rows, (long long)n, (long long)k);
   if (dx == nullptr && dw == nullptr && db == nullptr) return 0;
   NF_REQUIRE(dy && (db != nullptr || dw != nullptr || dx != nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE(dw == nullptr || (q && scale), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE(dx == nullptr || (w && (act == NF_ACT_NONE || (q && scale))), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE((rows == 1 || dy_stride >= n) && (n == 1 || dx == nullptr || w_stride >= k), NF_EINVAL, "row stride below the row's length");
   const KeepBwd p = keep_bwd(dy, dy_stride, w, w_stride, rows, n, k, dx != nullptr, dw != nullptr, db != nullptr);
+  NF_REQUIRE((p.dx.bm == 0 || tiles_fit(p.dx, rows, k)) && (p.dw.bm == 0 || tiles_fit(p.dw, n, k)), NF_EUNSUPPORTED,
+             "rows=%lld, n=%lld, k=%lld: more tiles than a launch holds", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(!p.narrow || ((uintptr_t)dx % 16 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)scale % 4 == 0), NF_EALIGN, "dx and q want 16-byte boundaries");
   NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
              "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
   hipStream_t s = (hipStream_t)stream;

@@ -357,7 +357,14 @@ __device__ __forceinline__ i32x4_t load16(const char* row, int at, int end) {
   return r;
 }
 
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // ---- host ---------------------------------------------------------------------------------------
+// A grid for `blocks` workgroups, of which one dimension alone could not hold them all: block_number() tells them apart; the last row of the grid may hold more.
+inline dim3 grid_of(int64_t blocks) {
+  const int64_t most = 1 << 20;
+  return blocks <= most ? dim3((unsigned)blocks) : dim3((unsigned)most, (unsigned)((blocks + most - 1) / most));
+}
 inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit * unit; }
 // whether rows of `bytes` with `ld` bytes between them can be read as they are; 256 of them stay inside 31 bits
 inline bool rows_fit(const void* p, int64_t ld, int64_t bytes) { return bytes % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
@@ -389,6 +396,10 @@ inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
   p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
   if (p.splits > 1) p.slot_bytes = round_up(p.splits * m * round_up(n, 8) * 4, 256);
   return p;
+}
+// whether one launch holds the plan's workgroups (of two threads for each row of a tile)
+inline bool tiles_fit(const TilePlan& p, int64_t m, int64_t n) {
+  return (double)((m + p.bm - 1) / p.bm) * (double)((n + p.bm - 1) / p.bm) * p.splits * (2 * p.bm) < 4294967296.0;
 }
 // copies rows to 16-byte boundaries, filled up with zeros to whole 16-byte pieces (int8_linear.hip)
 int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s);

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, 
 // rows copied to 16-byte boundaries and filled up with zeros, 16 bytes a thread
 __global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld, int bytes, char* to, int64_t rows) {
   const int pieces = (bytes + 15) / 16;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = block_number() * 256 + threadIdx.x;
   if (at >= rows * pieces) return;
   const int64_t row = at / pieces;
   const int k = (int)(at % pieces) * 16;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld,
 
 int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s) {
   const int64_t pieces = (bytes + 15) / 16;
-  hipLaunchKernelGGL(pack_rows_k, dim3((unsigned)((rows * pieces + 255) / 256)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
+  hipLaunchKernelGGL(pack_rows_k, grid_of((rows * pieces + 255) / 256), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
   return check_launch("pack_rows");
 }
 
@@ -237,7 +237,7 @@ int tile_launch(GemmArgs g, const Epilogue& e, int* slots, hipStream_t s) {
 using namespace nf;
 
 extern "C" int64_t nf_int8_linear_workspace_bytes(const int8_t* q, int64_t q_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k) {
-  if (rows <= 0 || n <= 0 || k <= 0 || rows >= (1ll << 31) || n >= (1ll << 31) || k > 131071) return 0;
+  if (rows <= 0 || n <= 0 || k <= 0 || rows >= (1ll << 31) || n > MOST_WIDTH || k > 131071) return 0;
   return plan(q, q_stride, w, w_stride, rows, n, k).total();
 }
 
@@ -247,13 +247,14 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   NF_REQUIRE(dtype_ok(y_dtype) && dtype_ok(bias_dtype), NF_EINVAL, "unknown dtype code");
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
   NF_REQUIRE(rows >= 0 && rows < (1ll << 31), NF_EINVAL, "rows=%lld outside 0..2^31-1", (long long)rows);
-  NF_REQUIRE(n >= 1 && n < (1ll << 31) - 256, NF_EINVAL, "n=%lld outside 1..2^31-257", (long long)n);
+  NF_REQUIRE(n >= 1 && n <= MOST_WIDTH, NF_EINVAL, "n=%lld outside 1..2^26", (long long)n);
   NF_REQUIRE(k >= 1, NF_EINVAL, "k=%lld below 1", (long long)k);
   NF_REQUIRE(k <= 131071, NF_EUNSUPPORTED, "k=%lld: more than 131071 products leave a 32-bit integer sum", (long long)k);
   if (rows == 0) return 0;
   NF_REQUIRE(q && scale && w && w_scale && y, NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE((rows == 1 || (q_stride >= k && y_stride >= n)) && (n == 1 || w_stride >= k), NF_EINVAL, "row stride below the row's length");
   const Plan p = plan(q, q_stride, w, w_stride, rows, n, k);
+  NF_REQUIRE(p.few || tiles_fit(p.tile, rows, n), NF_EUNSUPPORTED, "rows=%lld, n=%lld: more tiles than a launch holds", (long long)rows, (long long)n);
   NF_REQUIRE(p.total() == 0 || (workspace != nullptr && workspace_bytes >= p.total() && (uintptr_t)workspace % 16 == 0), NF_EINVAL,
              "this call needs a workspace of %lld bytes on a 16-byte boundary", (long long)p.total());
   hipStream_t s = (hipStream_t)stream;

@@ -90,7 +90,7 @@ __global__ __launch_bounds__(1024) void quantize_wide_k(Quantize a) {
 }
 
 template <typename XT, int ACT, bool KEEP>
-int quantize_launch(const Quantize& a, hipStream_t s) {
+int quantize_launch_some(const Quantize& a, hipStream_t s) {
   const auto go = [&](auto t_c, auto nv_c) {
     constexpr int T = decltype(t_c)::value, NV = decltype(nv_c)::value;
     const int64_t per = T < 256 ? 256 / T : 1;
@@ -109,6 +109,20 @@ int quantize_launch(const Quantize& a, hipStream_t s) {
   else if (a.width <= 32768) go(Int<1024>{}, Int<4>{});
   else hipLaunchKernelGGL((quantize_wide_k<XT, ACT, KEEP>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
   return check_launch("quantize_rows");
+}
+
+template <typename XT, int ACT, bool KEEP>
+int quantize_launch(const Quantize& a, hipStream_t s) {
+  typedef typename XT::storage X;
+  for (int64_t row = 0; row < a.rows; row += MOST_BLOCKS) {
+    Quantize part = a;
+    part.rows = a.rows - row < MOST_BLOCKS ? a.rows - row : MOST_BLOCKS;
+    part.x = (const X*)a.x + row * a.xs;
+    if (a.q != nullptr) part.q = a.q + row * a.width, part.scale = a.scale + row;
+    if (a.h != nullptr) part.h = (X*)a.h + row * a.hs;
+    if (const int rc = quantize_launch_some<XT, ACT, KEEP>(part, s)) return rc;
+  }
+  return 0;
 }
 
 template <typename XT>
@@ -132,7 +146,7 @@ extern "C" int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, in
   NF_REQUIRE(dtype_ok(x_dtype), NF_EINVAL, "unknown dtype code %d", x_dtype);
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
   NF_REQUIRE(rows >= 0 && rows < (1ll << 31), NF_EINVAL, "rows=%lld outside 0..2^31-1", (long long)rows);
-  NF_REQUIRE(width >= 1 && width <= (1 << 30), NF_EINVAL, "width=%lld outside 1..2^30", (long long)width);
+  NF_REQUIRE(width >= 1 && width <= MOST_WIDTH, NF_EINVAL, "width=%lld outside 1..2^26", (long long)width);
   NF_REQUIRE(h == nullptr || h_stride == width || h_stride == (width + 7) / 8 * 8, NF_EINVAL, "h_stride=%lld: the width, or the next multiple of 8",
              (long long)h_stride);
   if (rows == 0) return 0;

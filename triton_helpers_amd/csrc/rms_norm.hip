@@ -324,7 +324,7 @@ inline int64_t norm_groups(int64_t rows, int width) {
 }
 
 template <typename XT, typename RT>
-int fwd_launch(const NormFwd& a, bool eight, hipStream_t s) {
+int fwd_launch_some(const NormFwd& a, bool eight, hipStream_t s) {
   const auto go = [&](auto t_c, auto nv_c, auto e_c) {
     constexpr int T = decltype(t_c)::value, NV = decltype(nv_c)::value;
     constexpr bool E = decltype(e_c)::value != 0;
@@ -348,6 +348,24 @@ int fwd_launch(const NormFwd& a, bool eight, hipStream_t s) {
   if (eight) by_width(Int<1>{});
   else by_width(Int<0>{});
   return check_launch("rms_norm_fwd");
+}
+
+template <typename XT, typename RT>
+int fwd_launch(const NormFwd& a, bool eight, hipStream_t s) {
+  typedef typename XT::storage X;
+  typedef typename RT::storage R;
+  for (int64_t row = 0; row < a.rows; row += MOST_BLOCKS) {
+    NormFwd part = a;
+    part.rows = a.rows - row < MOST_BLOCKS ? a.rows - row : MOST_BLOCKS;
+    part.x = (const X*)a.x + row * a.xs;
+    if (a.r != nullptr) part.r = (const R*)a.r + row * a.rs;
+    if (a.h != nullptr) part.h = (R*)a.h + row * a.width;
+    part.y = (char*)a.y + row * a.width * (eight ? 1 : (int64_t)sizeof(X));
+    if (a.scale != nullptr) part.scale = a.scale + row;
+    if (a.rstd != nullptr) part.rstd = a.rstd + row;
+    if (const int rc = fwd_launch_some<XT, RT>(part, eight, s)) return rc;
+  }
+  return 0;
 }
 
 template <typename XT, typename HT>
@@ -383,7 +401,7 @@ extern "C" int nf_rms_norm_fwd(const void* x, int64_t x_stride, int x_dtype, con
   NF_REQUIRE(dtype_ok(x_dtype) && dtype_ok(residual_dtype) && dtype_ok(weight_dtype), NF_EINVAL, "unknown dtype code");
   NF_REQUIRE(residual_dtype == x_dtype || residual_dtype == NF_F32, NF_EUNSUPPORTED, "the residual is of the rows' type or float32");
   NF_REQUIRE(rows >= 0 && rows < (1ll << 31), NF_EINVAL, "rows=%lld outside 0..2^31-1", (long long)rows);
-  NF_REQUIRE(width >= 1 && width <= (1 << 30), NF_EINVAL, "width=%lld outside 1..2^30", (long long)width);
+  NF_REQUIRE(width >= 1 && width <= MOST_WIDTH, NF_EINVAL, "width=%lld outside 1..2^26", (long long)width);
   NF_REQUIRE(eps >= 0.0f, NF_EINVAL, "eps must be >= 0");
   if (rows == 0) return 0;
   NF_REQUIRE(x && y, NF_EINVAL, "NULL pointer argument");
@@ -399,7 +417,7 @@ extern "C" int nf_rms_norm_fwd(const void* x, int64_t x_stride, int x_dtype, con
 }
 
 extern "C" int64_t nf_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
-  if (rows <= 0 || width < 1 || width > (1 << 30)) return 0;
+  if (rows <= 0 || width < 1 || width > MOST_WIDTH) return 0;
   return slot_rows(rows, (int)width) * width * 4;
 }
 
@@ -409,7 +427,7 @@ extern "C" int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, c
   NF_REQUIRE(dtype_ok(x_dtype) && dtype_ok(h_dtype) && dtype_ok(weight_dtype), NF_EINVAL, "unknown dtype code");
   NF_REQUIRE(h_dtype == x_dtype || h_dtype == NF_F32, NF_EUNSUPPORTED, "the residual is of the rows' type or float32");
   NF_REQUIRE(rows >= 0 && rows < (1ll << 31), NF_EINVAL, "rows=%lld outside 0..2^31-1", (long long)rows);
-  NF_REQUIRE(width >= 1 && width <= (1 << 30), NF_EINVAL, "width=%lld outside 1..2^30", (long long)width);
+  NF_REQUIRE(width >= 1 && width <= MOST_WIDTH, NF_EINVAL, "width=%lld outside 1..2^26", (long long)width);
   NF_REQUIRE(dw == nullptr || weight != nullptr, NF_EINVAL, "a weight's gradient without a weight");
   if (rows == 0) {
     NF_REQUIRE(dw == nullptr, NF_EINVAL, "no rows: the weight's gradient is the caller's to clear");

@@ -124,6 +124,10 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
   return v;
 }
 
+// Rows go to launches of at most 2^21 workgroups (a grid of 2^32 threads is refused).
+constexpr int64_t MOST_BLOCKS = 1 << 21;
+constexpr int64_t MOST_WIDTH = 1 << 26;
+
 // ---- the 8-bit form of a row ----------------------------------------------------------------
 // q = rint(v * (127 / a)), s = a / 127, a the largest magnitude.  The magnitudes are compared as bit patterns, in which infinities come
 // behind every number and NaN behind them: a row that holds either has no 8-bit form, its scale becomes NaN and with it whatever is
