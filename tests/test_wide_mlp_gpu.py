@@ -134,6 +134,37 @@ def test_serving_a_token_captured():
         assert torch.equal(out, want[0]) and torch.equal(stream, want[1])
 
 
+def test_training_captured_and_an_eager_graph_refused():
+    """Two blocks' step replayed; while a graph of the same leaves from outside is alive, the captured forward refuses to begin."""
+    blocks = [_block(72, 160, torch.bfloat16), _block(72, 160, torch.bfloat16, "silu")]
+    leaves = [p for m in blocks for p in m.parameters()]
+    x, target = torch.randn(50, 72, device=DEV).bfloat16(), torch.randn(50, 72, device=DEV).bfloat16()
+
+    def forward():
+        out, stream = blocks[1](*blocks[0](x))
+        return out + stream
+
+    alive = forward()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside of this capture"):
+        with torch.cuda.graph(graph):
+            forward()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = forward()
+        grads = torch.autograd.grad(y, leaves, target)
+    for _ in range(3):
+        x.normal_()
+        target.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = forward()
+        assert torch.equal(y, want)
+        for a, b in zip(grads, torch.autograd.grad(want, leaves, target)):
+            assert torch.equal(a, b)
+
+
 def test_command_line(tmp_path):
     from triton_helpers.layers.wide_mlp.__main__ import main
 

@@ -5,6 +5,21 @@
 
 namespace {
 
+// An eager graph of a leaf that is still alive holds the node that adds up the leaf's gradient, on the stream that it was built on.  A backward that
+// is captured would end there: a stream outside of the capture has to wait for the captured one, and torch ends the process.
+// Refused in the forward, while nothing has happened yet.
+void refuse_eager_graph(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (node == nullptr || node->num_inputs() == 0) return;
+  const auto here = c10::hip::getCurrentHIPStream(t.device().index());
+  if (node->input_metadata(0).stream().id() == here.id() ||
+      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+    return;
+  TORCH_CHECK(false, "a graph that was built outside of this capture still holds one of the leaves: delete what it computed (outputs, losses) before capturing a "
+                     "step that takes gradients");
+}
+
 bool float_type(const Tensor& t) { return code_of(t.scalar_type()) >= 0; }
 
 // ------------------------------------------------------------------------------------------------ norm
@@ -130,6 +145,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release release;
     if (wants_grad(m)) {
+      for (const Tensor* t : {&m.x, &m.w, &m.r}) refuse_eager_graph(*t);
       const auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
       out = RmsNorm::apply(m.x, opt(m.w), opt(m.r), (double)m.eps);
     } else {
@@ -423,6 +439,7 @@ PyObject* checkpointed_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release release;
     if (needs_grad(m.x) || needs_grad(m.w) || needs_grad(m.b)) {
+      for (const Tensor* t : {&m.x, &m.w, &m.b}) refuse_eager_graph(*t);
       y = LinearKeep::apply(m.x, m.w, b, (int64_t)m.act, (int64_t)type);
     } else {
       const at::AutoDispatchBelowADInplaceOrView below;
