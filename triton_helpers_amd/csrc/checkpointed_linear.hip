@@ -21,8 +21,8 @@ struct Out {
   const int8_t* q;  // the gate's rows, without gaps
   const float* s;
   int m, n, y_dt;
-  float* sums;  // dW: partial sums of dy's columns [split][m], NULL where they are not wanted
-  void* db;     // ... or, of a single run, where they go, in type db_dt
+  float* sums;  // dW: partial sums of dy's columns [split][m] (of a single run: unused), NULL where they are not wanted
+  void* db;     // where they go, in type db_dt
   int db_dt;
 };
 
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
         float v = sums[i] + __shfl_xor(sums[i], 16);
         v += __shfl_xor(v, 32);
         if (lane < 16 && m + 16 * i < g.m) {
-          if (e.db != nullptr) store_any(e.db, m + 16 * i, e.db_dt, v);
+          if (slots == nullptr) store_any(e.db, m + 16 * i, e.db_dt, v);
           else e.sums[(int64_t)t.split * g.m + m + 16 * i] = v;
         }
       }
@@ -118,10 +118,21 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
   });
 }
 
+// the sums of the runs; dW's launch has workgroups for db's sums in front
+inline int64_t db_blocks(const Out& e) { return e.sums == nullptr ? 0 : (e.m + 255) / 256; }
 template <typename T, int MODE>
-__global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits, Out e) {
+__global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits, Out e, int db_blocks) {
+  if (MODE == OUT_PLAIN && (int)blockIdx.x < db_blocks) {
+    const int m = blockIdx.x * 256 + threadIdx.x;
+    if (m >= e.m) return;
+    float v = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) v += e.sums[(int64_t)k * e.m + m];
+    store_any(e.db, m, e.db_dt, v);
+    return;
+  }
   const int64_t parts = (e.n + 7) / 8, ld = parts * 8, each = (int64_t)e.m * ld;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = (int64_t)(blockIdx.x - db_blocks) * 256 + threadIdx.x;
   if (at >= e.m * parts) return;
   const int m = (int)(at / parts), n = (int)(at % parts) * 8;
   float v[8] = {}, b[8] = {};
@@ -139,7 +150,7 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
 }
 
 // What the backward's products read and the caller does not have: copies of dy and W on 16-byte boundaries, and act(s q) in 16 bits, each with rows
-// filled up with zeros to whole 16-byte pieces.  A stream, 16 bytes a thread; one launch for all of them (of what a small layer's step takes,
+// filled up with zeros to whole 16-byte pieces.  Streams, 16 bytes a thread and store; one launch for all of them (of what a small layer's step takes,
 // launches are the most).
 struct Copy {
   const char* from;
@@ -156,52 +167,66 @@ struct Prepare {
   int64_t rows;
   int width, act;
 };
-template <typename T>
+template <typename T, int J>
 __global__ __launch_bounds__(256) void prepare_k(Prepare a) {
   int64_t block = block_number();
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (block < a.copy[c].blocks) {
       const Copy& m = a.copy[c];
-      const int pieces = (m.bytes + 15) / 16;
-      const int64_t at = block * 256 + threadIdx.x;
-      if (at >= m.rows * pieces) return;
-      const int64_t row = at / pieces;
-      const int k = (int)(at - row * pieces) * 16;
-      *(i32x4_t*)(m.to + at * 16) = load16(m.from + row * m.ld, k, m.bytes);
+      copy_rows<J>(block, m.from, m.ld, m.bytes, m.to, m.rows);
       return;
     }
     block -= a.copy[c].blocks;
   }
-  const int pieces = (a.width + 7) / 8;
-  const int64_t at = block * 256 + threadIdx.x;
-  if (at >= a.rows * pieces) return;
-  const int64_t row = at / pieces;
-  const int c = (int)(at - row * pieces) * 8, n = a.width - c;
-  const int8_t* p = a.q + row * a.width + c;
-  int8_t raw[8];
-  if (n >= 8) __builtin_memcpy(raw, p, 8);
-  else
+  const Cut<J> cut(block, (a.width + 7) / 8);
+  int q[J][2];
+  float scale[J];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = i < n ? p[i] : (int8_t)0;
-  const float scale = a.s[row];
+  for (int j = 0; j < J; ++j) {
+    int piece;
+    const int64_t row = cut.row(j, &piece);
+    const int n = a.width - piece * 8;
+    q[j][0] = q[j][1] = 0;
+    scale[j] = 0.0f;
+    if (row < a.rows) {
+      const int8_t* p = a.q + row * a.width + piece * 8;
+      if (n >= 8) {
+        __builtin_memcpy(q[j], p, 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (i < n) q[j][i / 4] |= (p[i] & 255) << (i % 4 * 8);
+      }
+      scale[j] = a.s[row];
+    }
+  }
   with_act(a.act, [&](auto act_c) {
-    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? act_value<decltype(act_c)::value>(scale * (float)raw[i]) : 0.0f;
-    store8<T>(a.h + at * 8, 8, v);
+    for (int j = 0; j < J; ++j) {
+      int piece;
+      const int64_t row = cut.row(j, &piece);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = scale[j] * (float)(q[j][i / 4] << (24 - i % 4 * 8) >> 24);
+        v[i] = piece * 8 + i < a.width ? act_value<decltype(act_c)::value>(x) : 0.0f;
+      }
+      if (row < a.rows) store8<T>(a.h + (row * cut.each + piece) * 8, 8, v);
+    }
   });
 }
 
-// partial column sums: a workgroup takes 256 columns of rows 8 group + 0..7, and every 8 groups on
+// Partial column sums: `across` threads (32 or 64) side by side, eight columns each, the others below; the workgroups of a strip take turns at the rows.  16384 x
+// 4096 bf16: 43 us with 64 threads across and 2048 workgroups, 51 with 32, 56 with 1024 workgroups, 50 with 256.
 template <typename T>
-__global__ __launch_bounds__(256) void column_sums_k(const uint16_t* dy, int64_t ld, int64_t rows, int n, float* slots) {
-  __shared__ float part[8][256];
-  const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8, r = threadIdx.x >> 5;
+__global__ __launch_bounds__(256) void column_sums_k(const uint16_t* dy, int64_t ld, int64_t rows, int n, int across, float* slots) {
+  __shared__ float part[8 * 256];
+  const int t = threadIdx.x & (across - 1), c = (blockIdx.x * across + t) * 8, r = threadIdx.x / across, down = 256 / across;
   float s[8] = {};
   if (c < n) {
-#pragma unroll 4
-    for (int64_t row = blockIdx.y * 8 + r; row < rows; row += gridDim.y * 8) {
+#pragma unroll 8
+    for (int64_t row = blockIdx.y * down + r; row < rows; row += gridDim.y * down) {
       float v[8];
       load8<T>(dy + row * ld + c, n - c, v);
 #pragma unroll
@@ -209,14 +234,15 @@ __global__ __launch_bounds__(256) void column_sums_k(const uint16_t* dy, int64_t
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[r][(threadIdx.x & 31) * 8 + i] = s[i];
+  for (int i = 0; i < 8; ++i) part[(r * across + t) * 8 + i] = s[i];
   __syncthreads();
-  const int column = blockIdx.x * 256 + threadIdx.x;
-  if (column >= n) return;
-  float v = part[0][threadIdx.x];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) v += part[i][threadIdx.x];
-  slots[(int64_t)blockIdx.y * n + column] = v;
+  for (int j = threadIdx.x; j < across * 8; j += 256) {
+    const int column = blockIdx.x * across * 8 + j;
+    if (column >= n) break;
+    float v = part[j];
+    for (int i = 1; i < down; ++i) v += part[i * across * 8 + j];
+    slots[(int64_t)blockIdx.y * n + column] = v;
+  }
 }
 
 template <typename T, int MODE, bool AX, bool BX>
@@ -237,8 +263,13 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
   else go(Int<256>{}, Int<4>{}, Int<2>{});
   const int rc = check_launch("checkpointed_linear");
   if (rc != 0 || p.splits == 1) return rc;
-  if (MODE == OUT_PLAIN && e.n % 8 == 0 && (int64_t)e.m * e.n < (1ll << 31)) return sum_slots(slots, p.splits, (int64_t)e.m * e.n, e.y, e.y_dt, s);
-  hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)((e.m * (int64_t)((e.n + 7) / 8) + 255) / 256)), dim3(256), 0, s, slots, p.splits, e);
+  // (many runs: over several threads)
+  if (MODE == OUT_PLAIN && e.n % 8 == 0 && p.splits > 8) {
+    const int rc = sum_slots(slots, p.splits, (int64_t)e.m * e.n, e.y, e.y_dt, s);
+    return rc != 0 || e.sums == nullptr ? rc : sum_slots(e.sums, p.splits, e.m, e.db, e.db_dt, s);
+  }
+  const int64_t first = db_blocks(e), blocks = first + (e.m * (int64_t)((e.n + 7) / 8) + 255) / 256;
+  hipLaunchKernelGGL((keep_sum_k<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, s, slots, p.splits, e, (int)first);
   return check_launch("checkpointed_linear_sum");
 }
 
@@ -266,7 +297,7 @@ KeepFwd keep_fwd(const void* x, int64_t xs, const void* w, int64_t ws, int64_t r
 struct KeepBwd {
   bool narrow;
   int64_t ldk, ldn, dy_bytes, w_bytes, h_bytes, sum_bytes;
-  int strips, groups;
+  int across, strips, groups;
   bool sums_in_dw;
   TilePlan dx, dw;
   int64_t slots() const { return dx.slot_bytes > dw.slot_bytes ? dx.slot_bytes : dw.slot_bytes; }
@@ -295,8 +326,9 @@ KeepBwd keep_bwd(const void* dy, int64_t dys, const void* w, int64_t ws, int64_t
   if (p.sums_in_dw) {
     if (p.dw.splits > 1) p.sum_bytes = round_up((int64_t)p.dw.splits * n * 4, 256);
   } else if (need_db) {
-    p.strips = (int)((n + 255) / 256);
-    const int64_t most = 1024 / p.strips + 1, want = (rows + 63) / 64;
+    p.across = n <= 256 ? 32 : 64;
+    p.strips = (int)((n + 8 * p.across - 1) / (8 * p.across));
+    const int64_t most = 2048 / p.strips + 1, want = (rows + 63) / 64;
     p.groups = (int)(want < most ? want : most);
     p.sum_bytes = round_up((int64_t)p.groups * n * 4, 256);
   }
@@ -333,24 +365,26 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
     return sum_slots(part_dw, p.groups, n * k, dw, dw_dt, s);
   }
   if (db != nullptr && !p.sums_in_dw) {
-    hipLaunchKernelGGL((column_sums_k<T>), dim3(p.strips, p.groups), dim3(256), 0, s, (const uint16_t*)dy, dys, rows, (int)n, (float*)sums);
+    hipLaunchKernelGGL((column_sums_k<T>), dim3(p.strips, p.groups), dim3(256), 0, s, (const uint16_t*)dy, dys, rows, (int)n, p.across, (float*)sums);
     if (const int rc = check_launch("column_sums")) return rc;
     if (const int rc = sum_slots((const float*)sums, p.groups, n, db, db_dt, s)) return rc;
   }
   Prepare make{};
   int64_t blocks = 0;
+  const int each = cut_pieces((p.dy_bytes + p.w_bytes + p.h_bytes) / 16);
   const auto copy = [&](int i, const void* from, int64_t ld, int64_t count, int64_t width, char* to) {
-    make.copy[i] = {(const char*)from, ld * 2, count, to, (int)width * 2, (count * ((width + 7) / 8) + 255) / 256};
+    make.copy[i] = {(const char*)from, ld * 2, count, to, (int)width * 2, cut_blocks(count * ((width + 7) / 8), each)};
     blocks += make.copy[i].blocks;
   };
   if (p.dy_bytes > 0) copy(0, dy, dys, rows, n, packed_dy);
   if (p.w_bytes > 0) copy(1, w, ws, n, k, packed_w);
   if (dw != nullptr) {
     make.q = q, make.s = scale, make.h = (uint16_t*)h, make.rows = rows, make.width = (int)k, make.act = act;
-    blocks += (rows * (p.ldk / 8) + 255) / 256;
+    blocks += cut_blocks(rows * (p.ldk / 8), each);
   }
   if (blocks > 0) {
-    hipLaunchKernelGGL((prepare_k<T>), grid_of(blocks), dim3(256), 0, s, make);
+    if (each == 1) hipLaunchKernelGGL((prepare_k<T, 1>), grid_of(blocks), dim3(256), 0, s, make);
+    else hipLaunchKernelGGL((prepare_k<T, 4>), grid_of(blocks), dim3(256), 0, s, make);
     if (const int rc = check_launch("checkpointed_linear_prepare")) return rc;
   }
   const char* a = p.dy_bytes > 0 ? packed_dy : (const char*)dy;
@@ -362,11 +396,8 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
   }
   if (dw != nullptr) {
     const GemmArgs g{a, h, lda, p.ldk * 2, (int)n, (int)k, (int)rows * 2, 0, 0, 0, 0};
-    const bool once = p.dw.splits == 1;
-    const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt, p.sums_in_dw ? (float*)sums : nullptr, once ? db : nullptr, db_dt};
-    if (const int rc = product<T, OUT_PLAIN, true, true>(g, p.dw, e, slots, s)) return rc;
-    if (p.sums_in_dw && !once)
-      if (const int rc = sum_slots((const float*)sums, p.dw.splits, n, db, db_dt, s)) return rc;
+    const Out e{dw, k, nullptr, NF_F32, NF_ACT_NONE, nullptr, nullptr, (int)n, (int)k, dw_dt, p.sums_in_dw ? (float*)sums : nullptr, db, db_dt};
+    return product<T, OUT_PLAIN, true, true>(g, p.dw, e, slots, s);
   }
   return 0;
 }

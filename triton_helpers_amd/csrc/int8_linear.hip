@@ -188,19 +188,15 @@ __global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, 
   with_epilogue(e, [&](auto act_c, auto y_c) { put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, sum, s, columns); });
 }
 
-// rows copied to 16-byte boundaries and filled up with zeros, 16 bytes a thread
+template <int J>
 __global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld, int bytes, char* to, int64_t rows) {
-  const int pieces = (bytes + 15) / 16;
-  const int64_t at = block_number() * 256 + threadIdx.x;
-  if (at >= rows * pieces) return;
-  const int64_t row = at / pieces;
-  const int k = (int)(at % pieces) * 16;
-  *(i32x4_t*)(to + row * pieces * 16 + k) = load16(from + row * ld, k, bytes);
+  copy_rows<J>(block_number(), from, ld, bytes, to, rows);
 }
 
 int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s) {
   const int64_t pieces = (bytes + 15) / 16;
-  hipLaunchKernelGGL(pack_rows_k, grid_of((rows * pieces + 255) / 256), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
+  if (cut_pieces(rows * pieces) == 1) hipLaunchKernelGGL((pack_rows_k<1>), grid_of(cut_blocks(rows * pieces, 1)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
+  else hipLaunchKernelGGL((pack_rows_k<4>), grid_of(cut_blocks(rows * pieces, 4)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
   return check_launch("pack_rows");
 }
 
