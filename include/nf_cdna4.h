@@ -1,6 +1,7 @@
 /*
  * nf_cdna4.h -- C ABI of libnf_cdna4.so: hand-written gfx950 (MI355X) kernels for
- * the three neural-field hot paths of triton_helpers.layers.
+ * the three neural-field hot paths of triton_helpers.layers, and for the layers
+ * of wider networks (norm, 8-bit rows and products).
  *
  * Every entry point takes raw device pointers, sizes and strides in ELEMENTS,
  * dtype codes and a HIP stream handle (hipStream_t passed as void*; NULL = the
@@ -33,7 +34,7 @@
 extern "C" {
 #endif
 
-#define NF_ABI_VERSION 9
+#define NF_ABI_VERSION 10
 
 /* element types */
 enum { NF_F32 = 0, NF_F16 = 1, NF_BF16 = 2 };

@@ -15,7 +15,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libnf_cdna4.so"
 NATIVE_PATH = LIB_PATH.with_name("_native.so")
 
-NF_ABI_VERSION = 9
+NF_ABI_VERSION = 10
 NF_F32, NF_F16, NF_BF16 = 0, 1, 2
 NF_ACT = {"none": 0, "relu": 1, "silu": 2, "relu2": 3, "gelu": 4}
 NF_MAX_LEVELS = 32

@@ -8,7 +8,10 @@
 // registers and reads the next half's between the matrix instructions.  There is one meeting of the waves in a step, behind its first half: then
 // all of the step is in registers, its two slots are free, and the next step has to be there.
 //
-// bf16 16384 x 4096 x 4096 on tiles of 256 x 256: RATE_NT
+// On tiles of 256 x 256: bf16 16384 x 4096 x 4096 along the sum 395 us alone, 408 - 425 in a training step (1290 - 1390 TFLOP/s), both operands crosswise 396 - 415;
+// int8 16384 x 8192 x 8192 820 us (2680 Tops/s).  The matrix units are busy for 70 % of the clocks (74 % crosswise, int8 69 %), at some 1.9 GHz; what
+// bounds the rest is the loads: without them (their data stale) 1730 TFLOP/s.  Measured and not kept: matrix instructions of 32x32, 3 to 10 % slower; 64-byte steps
+// with a meeting every second one, 12 %; priorities for the waves that multiply, -4 to +7 %; groups of 2, 8 or 16 row tiles, up to 10 %.
 //
 // Rows start on 16-byte boundaries and hold whole 16-byte pieces (along the summed dimension: with zeros behind the last value).  Rows of C beyond
 // the operand repeat its last one, columns of a crosswise operand beyond it are whatever the buffer holds: neither is stored.  What lies
@@ -336,7 +339,7 @@ __device__ __forceinline__ void vector8(const void* p, int dt, int n, int count,
 }
 
 // 16 bytes of a row from any address; bytes beyond the row's end are zeros.  A piece that reaches over the end is read as the row's last 16 bytes
-// and shifted (byte by byte it took longer than all of a short product: 19 x 5000 x 4098 18 us instead of 13.6).
+// and shifted (byte by byte that took longer than all the rest of a short product: 19 x 5000 x 4098 18.2 us instead of 13.6).
 __device__ __forceinline__ i32x4_t load16(const char* row, int at, int end) {
   uint64_t v[2] = {0, 0};
   if (end >= 16) {

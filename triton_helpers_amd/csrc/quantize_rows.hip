@@ -1,7 +1,8 @@
 // Rows as 8-bit integers with one scale each, q = rint(v (127 / a)) and s = a / 127 with a the largest magnitude of the row, and next to them, on
 // request, act(v) in the rows' own type with rows padded to whole 16-byte pieces (the operand of the product that the rows go into).
 //
-// A stream over HBM: a row is read once and held in registers between its maximum and its rounding; rows above 32768 values are read twice.
+// A stream over HBM: a row is read once and held in registers between its maximum and its rounding; rows above 32768 values are read twice.  Short rows
+// share a wave (2^18 x 256 57 us instead of 107).  16384 x 4096 bf16 with GELU: 61 us, 335 MB at 5.5 TB/s.
 #include "wide_common.h"
 
 namespace nf {

@@ -6,7 +6,11 @@
 // A stream over HBM: a row is read once, held in registers as float32 through its sums, and written once.  Up to 2048 values a row belongs to
 // one wave (sums by lane exchange, no barrier), beyond that to a workgroup; rows that do not fit the registers (above 32768 values, 16384 in the
 // backward) are read twice.
-// The norm is taken of the unrounded sum; the backward sees the rounded one that was kept.
+// The norm is taken of the unrounded sum; the backward sees the rounded one that was kept (the new residual, which is there anyway: keeping x and the old
+// residual in its place would cost a tensor of memory and a ninth of the traffic, and makes a 16-bit dw, whose own rounding is as large, 1.4 times as exact).
+//
+// 16384 x 4096 bf16 with a residual: forward 96 us (537 MB, 5.6 TB/s; a large copy reaches 4.9, part of this comes out of the memory-side cache), backward 127
+// and the sum of its dw 5 (4.2 TB/s); with autograd 229 a step.  5003 x 777 float32: 10.4, 12.5 and 4.2, and the host's 56 a step.  1 x 4096: 2.8, 6.3 a call.
 #include "wide_common.h"
 
 namespace nf {
