@@ -328,8 +328,8 @@ int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const 
  *   forward   y[m, n] = sum_k act(x[m, k]) w[n, k] + bias[n];  q, scale: the 8-bit rows of x (NULL both: nothing is kept)
  *   backward  x^ = scale q;  dx = (dy w) * act'(x^);  dw = dy^T act(x^);  db = column sums of dy; each written, each may be NULL
  * Sums in float32; act(x) and act(x^) enter the products rounded to the rows' type.  bias and db of any type, dw of the rows' type or float32.  dx and
- * q [rows, k] and dw [n, k] without gaps; y, q and dx on 16-byte boundaries, y's rows too where n is a multiple of 8.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and
- * strides).  Results are the same bits on every run.  The backward wants at least one row; w may be NULL without dx, q and scale where
+ * q [rows, k] and dw [n, k] without gaps; y, q and dx on 16-byte boundaries, y's rows too where n is a multiple of 8.  Up to 2^29 rows and 2^20 channels
+ * on either side.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and strides).  Results are the same bits on every run.  The backward wants at least one row; w may be NULL without dx, q and scale where
  * neither dw nor an activation's dx needs them. */
 int64_t nf_linear_keep_fwd_workspace_bytes(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows, int64_t n, int64_t k, int act);
 int nf_linear_keep_fwd(const void* x, int64_t x_stride, int dtype, const void* w, int64_t w_stride, const void* bias, int bias_dtype, void* y,

@@ -151,7 +151,7 @@ def test_keep_entry_points():
     refused(fwd(dt=F32), -2, b"float16 or bfloat16")
     refused(fwd(bdt=5), -1, b"dtype")
     refused(fwd(act=7), -1, b"activation")
-    for bad in ({"rows": 2**30}, {"rows": -1}, {"n": 0}, {"k": 0}, {"k": 2**26 + 1}, {"n": 2**26 + 1}):
+    for bad in ({"rows": 2**30}, {"rows": -1}, {"n": 0}, {"k": 0}, {"k": 2**20 + 1}, {"n": 2**20 + 1}, {"k": 2**22}):
         refused(fwd(**bad), -1, b"rows")
     refused(fwd(w=None), -1, b"NULL")
     refused(fwd(s=None), -1, b"NULL")
@@ -192,6 +192,7 @@ def test_keep_entry_points():
     assert big >= 128 * 48 * (64 + 1) * 4
     refused(bwd(rows=4096, dx=24, work=16, size=big), -3, b"boundaries")
     refused(bwd(rows=4096, work=16, size=big - 1), -1, b"workspace")
+    refused(bwd(k=2**20 + 8, ws=2**20 + 8, work=16, size=2**62), -1, b"2^20")
     refused(bwd(rows=2**29, k=2**20, ws=2**20, n=264, ds=264, work=16, size=2**62), -2, b"more tiles")
 
 

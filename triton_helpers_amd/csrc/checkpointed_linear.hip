@@ -278,8 +278,10 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
   return check_launch("checkpointed_linear_sum");
 }
 
+// (256 rows of a copied operand stay inside 31 bits, as rows_fit asks of the caller's own)
+constexpr int64_t MOST_CHANNELS = 1 << 20;
 inline bool sizes_ok(int64_t rows, int64_t n, int64_t k) {
-  return rows > 0 && rows <= (1ll << 29) && n >= 1 && n <= MOST_WIDTH && k >= 1 && k <= MOST_WIDTH;
+  return rows > 0 && rows <= (1ll << 29) && n >= 1 && n <= MOST_CHANNELS && k >= 1 && k <= MOST_CHANNELS;
 }
 
 struct KeepFwd {
@@ -423,7 +425,7 @@ extern "C" int nf_linear_keep_fwd(const void* x, int64_t x_stride, int dtype, co
   NF_REQUIRE(dtype_ok(bias_dtype), NF_EINVAL, "unknown dtype code %d", bias_dtype);
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
   if (rows == 0) return 0;
-  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows up to 2^29, channels 1..2^26", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows up to 2^29, channels 1..2^20", (long long)rows, (long long)n, (long long)k);
   NF_REQUIRE(x && w && y && (q == nullptr) == (scale == nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE((rows == 1 || (x_stride >= k && y_stride >= n)) && (n == 1 || w_stride >= k), NF_EINVAL, "row stride below the row's length");
   const KeepFwd p = keep_fwd(x, x_stride, w, w_stride, rows, n, k, act);
@@ -447,7 +449,7 @@ extern "C" int nf_linear_keep_bwd(const void* dy, int64_t dy_stride, int dtype, 
   NF_REQUIRE(dtype == NF_F16 || dtype == NF_BF16, NF_EUNSUPPORTED, "dtype code %d: float16 or bfloat16 rows", dtype);
   NF_REQUIRE((dw_dtype == dtype || dw_dtype == NF_F32) && dtype_ok(db_dtype), NF_EUNSUPPORTED, "the weight's gradient is of the rows' type or float32");
   NF_REQUIRE(act >= NF_ACT_NONE && act <= NF_ACT_GELU, NF_EINVAL, "unknown activation %d", act);
-  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows 1..2^29, channels 1..2^26", (long long)rows, (long long)n, (long long)k);
+  NF_REQUIRE(sizes_ok(rows, n, k), NF_EINVAL, "rows=%lld, n=%lld, k=%lld: rows 1..2^29, channels 1..2^20", (long long)rows, (long long)n, (long long)k);
   if (dx == nullptr && dw == nullptr && db == nullptr) return 0;
   NF_REQUIRE(dy && (db != nullptr || dw != nullptr || dx != nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE(dw == nullptr || (q && scale), NF_EINVAL, "NULL pointer argument");
