@@ -102,24 +102,16 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_fwd_k(NarrowFwd a) {
       const auto to_s = rows_of(a.scale, tile * TILE, a.rows, 4, 4);
       uint32_t top[EACH];
 #pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        top[j] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t m = magnitude_bits(v[j][i]);
-          top[j] = top[j] > m ? top[j] : m;
-        }
-      }
+      for (int j = 0; j < EACH; ++j) top[j] = largest16({(uint32_t)x[j][0], (uint32_t)x[j][1], (uint32_t)x[j][2], (uint32_t)x[j][3]});
 #pragma unroll
       for (int j = 0; j < EACH; ++j) top[j] = lanes_max<PIECES>(top[j]);
 #pragma unroll
       for (int j = 0; j < EACH; ++j) {
         const int r = r0 + j * ROWS;
-        const EightBit e = eight_bit(top[j]);
-        u32x2_t q = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i / 4] |= ((uint32_t)(int)quantized(v[j][i], e) & 255u) << (i % 4 * 8);
-        __builtin_amdgcn_raw_buffer_store_b64(q, to_q, in ? r * a.k + p * 8 : NOWHERE, 0, 0);
+        const EightBit e = eight_bit(magnitude_bits(T::to_f32((uint16_t)top[j])));
+        uint32_t q[2];
+        quantized8<true>(v[j], e, q);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{q[0], q[1]}, to_q, in ? r * a.k + p * 8 : NOWHERE, 0, 0);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(e.scale), to_s, p == 0 ? r * 4 : NOWHERE, 0, 0);
       }
     }
@@ -229,8 +221,7 @@ __global__ __launch_bounds__(THREADS, 2) void narrow_bwd_k(NarrowBwd a) {
 #pragma unroll
     for (int j = 0; j < EQ; ++j) {
       float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = s[j] * (float)(q[j][i / 4] << (24 - i % 4 * 8) >> 24);
+      kept8(q[j], s[j], v);
       with_act(a.act, [&](auto act_c) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(act_c)::value>(v[i]);

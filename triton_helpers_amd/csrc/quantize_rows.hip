@@ -56,9 +56,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_k(Quantize a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * T + t) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] = quantized(v[j][i], e);
-    store8_q(a.q + row * a.width + c, a.width - c, v[j]);
+    store8_q<sizeof(typename XT::storage) == 2>(a.q + row * a.width + c, a.width - c, v[j], e);
   }
 }
 
@@ -84,9 +82,7 @@ __global__ __launch_bounds__(1024) void quantize_wide_k(Quantize a) {
   for (int c = threadIdx.x * 8; c < a.width; c += 8192) {
     float v[8];
     load8<XT>(x + c, a.width - c, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = quantized(v[i], e);
-    store8_q(a.q + row * a.width + c, a.width - c, v);
+    store8_q<sizeof(typename XT::storage) == 2>(a.q + row * a.width + c, a.width - c, v, e);
   }
 }
 

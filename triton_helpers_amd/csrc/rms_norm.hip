@@ -90,9 +90,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_fwd_k(NormFwd a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * T + t) * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] = quantized(h[j][i], e);
-      store8_q(o + c, a.width - c, h[j]);
+      store8_q<false>(o + c, a.width - c, h[j], e);
     }
   } else {
     auto* o = (typename XT::storage*)a.y + row * a.width;
@@ -158,9 +156,7 @@ __global__ __launch_bounds__(1024) void rms_fwd_wide_k(NormFwd a) {
     float h[8];
     normed_at(c, h);
     if constexpr (EIGHT) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = quantized(h[i], e);
-      store8_q((int8_t*)a.y + row * a.width + c, a.width - c, h);
+      store8_q<false>((int8_t*)a.y + row * a.width + c, a.width - c, h, e);
     } else {
       store8<XT>((typename XT::storage*)a.y + row * a.width + c, a.width - c, h);
     }

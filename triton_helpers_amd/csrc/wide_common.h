@@ -53,18 +53,6 @@ __device__ __forceinline__ void store_any(void* p, int64_t at, int dt, float v) 
   if (dt == NF_F32) ((float*)p)[at] = v;
   else ((uint16_t*)p)[at] = dt == NF_F16 ? F16::from_f32(v) : BF16::from_f32(v);
 }
-__device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&q)[8]) {
-  int8_t raw[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) raw[i] = (int8_t)(int)q[i];
-  if (n >= 8) {
-    __builtin_memcpy(p, raw, 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) p[i] = raw[i];
-  }
-}
 
 // ---- over the T threads of a row (up to 64: neighbouring lanes of a wave; else the whole workgroup) -----------------
 // (lane exchanges inside the vector unit: through LDS each costs some hundred clocks, one behind the other)
@@ -142,8 +130,50 @@ __device__ __forceinline__ EightBit eight_bit(uint32_t largest) {
   if (a < 7.5231638e-37f) return {0.0f, 0.0f};
   return {a / 127.0f, 127.0f / a};
 }
-// of a row with a scale; NaN and infinities (inverse = 0) become zeros
-__device__ __forceinline__ float quantized(float v, EightBit e) { return e.inverse == 0.0f ? 0.0f : rintf(v * e.inverse); }
+// Eight values of a row as bytes.  What is added puts the product, rounded to a whole number (half to even, as rint does), into the low byte of its bits.  In a row
+// without a form (inverse = 0) infinities and NaN become zeros: NaN that came from 16 bits, and those of the chip, have nothing in their low byte.
+template <bool FROM16>
+__device__ __forceinline__ void quantized8(const float (&v)[8], EightBit e, uint32_t (&q)[2]) {
+#pragma clang fp contract(off)
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float product = v[i] * e.inverse;
+    b[i] = __float_as_uint(product + 12582912.0f);
+    if (!FROM16 && e.inverse == 0.0f) b[i] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x0c0c0400u);
+    q[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  }
+}
+template <bool FROM16>
+__device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&v)[8], EightBit e) {
+  uint32_t q[2];
+  quantized8<FROM16>(v, e, q);
+  if (n >= 8) {
+    __builtin_memcpy(p, q, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = (int8_t)(q[i / 4] >> (i % 4 * 8));
+  }
+}
+// ... and back: s q.  (A byte less 128 as one multiplication and addition: 128 s is exact, so is nothing rounded but the result.)
+__device__ __forceinline__ void kept8(const int (&q)[2], float s, float (&v)[8]) {
+  const float shift = -128.0f * s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = fmaf((float)(uint8_t)(((uint32_t)q[i / 4] ^ 0x80808080u) >> (i % 4 * 8)), s, shift);
+}
+// the largest magnitude of eight 16-bit values, in their type's bits
+__device__ __forceinline__ uint16_t largest16(const uint32_t (&v)[4]) {
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu));
+  return m[0] > m[1] ? m[0] : m[1];
+}
 
 // ---- activations ------------------------------------------------------------------------------
 // As act_fwd / act_grad, which are made for 16-bit results, but for a GELU that is right to 1.5e-7, and a NaN stays one.
