@@ -36,11 +36,11 @@ struct Gate {
   int q[2];
   float s;
 };
-template <int ACT>
+template <bool GATE>
 __device__ __forceinline__ Gate gate_of(const Out& e, int m, int n) {
   Gate g{};
-  if constexpr (ACT != NF_ACT_NONE) {
-    if (m < e.m && n < e.n) {
+  if constexpr (GATE) {
+    if (e.act != NF_ACT_NONE && m < e.m && n < e.n) {
       const int8_t* q = e.q + (int64_t)m * e.n + n;
       const int left = e.n - n;
       if (left >= 8) {
@@ -78,7 +78,7 @@ __device__ __forceinline__ void with_out(const Out& e, Body&& body) {
 }
 
 template <typename T, typename G, int MODE>
-__global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, float* slots) {
+__global__ __launch_bounds__(G::THREADS, G::WAVES_SIMD) void keep_tile_k(GemmArgs g, Out e, float* slots) {
   __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
   f32x4_t acc[G::FM][G::FN] = {};
   const Tile t = tile_of(g, blockIdx.x);
@@ -108,17 +108,20 @@ __global__ __launch_bounds__(G::THREADS, 2) void keep_tile_k(GemmArgs g, Out e, 
   if (slots != nullptr) {  // [split][m][n rounded up to 8]
     const int64_t ld = (g.n + 7) / 8 * 8;
     float* o = slots + (int64_t)t.split * g.m * ld + n;
-    G::each8(t, lds, acc, [](int) { return 0; }, [&](int m, const float (&v)[8], int) {
-      if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+    G::each8(t, lds, acc, [](int) { return 0; }, [&](auto&& rows) {
+      rows([&](int m, const float (&v)[8], int) {
+        if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+      });
     });
     return;
   }
   float b[8] = {};
   if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
-  with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
-    constexpr int ACT = decltype(act_c)::value;
-    G::each8(t, lds, acc, [&](int m) { return gate_of<MODE == OUT_GATE ? ACT : NF_ACT_NONE>(e, m, n); }, [&](int m, const float (&v)[8], const Gate& gate) {
-      if (m < g.m && n < g.n) put8<MODE, ACT, decltype(y_c)>(e, m, n, v, b, gate);
+  G::each8(t, lds, acc, [&](int m) { return gate_of<MODE == OUT_GATE>(e, m, n); }, [&](auto&& rows) {
+    with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
+      rows([&](int m, const float (&v)[8], const Gate& gate) {
+        if (m < g.m && n < g.n) put8<MODE, decltype(act_c)::value, decltype(y_c)>(e, m, n, v, b, gate);
+      });
     });
   });
 }
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
   if (MODE == OUT_BIAS && e.bias != nullptr) vector8(e.bias, e.bias_dt, n, e.n, b);
   with_out<MODE, T>(e, [&](auto act_c, auto y_c) {
     constexpr int ACT = decltype(act_c)::value;
-    put8<MODE, ACT, decltype(y_c)>(e, m, n, v, b, gate_of<MODE == OUT_GATE ? ACT : NF_ACT_NONE>(e, m, n));
+    put8<MODE, ACT, decltype(y_c)>(e, m, n, v, b, gate_of<MODE == OUT_GATE>(e, m, n));
   });
 }
 
@@ -262,10 +265,11 @@ int product(GemmArgs g, const TilePlan& p, const Out& e, float* slots, hipStream
     hipLaunchKernelGGL((keep_tile_k<T, G, MODE>), dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(G::THREADS), 0, s, g, e,
                        p.splits > 1 ? slots : nullptr);
   };
-  // (waves of 64 x 128 are 2 % quicker than 128 x 64 where both operands lie along the sum, 2 to 5 % slower where one is crosswise)
+  // (16384 x 4096 x 4096: where both operands lie along the sum four waves of 128 x 128, which read LDS three quarters as often, take 400 us at best, eight of 64 x 128
+  // 410, of 128 x 64 2 % more; where one is crosswise eight of 128 x 64 take 440 and 400, of 64 x 128 2 to 5 % more, four 510 and 410)
   if (p.bm == 128) go(Int<128>{}, Int<2>{}, Int<2>{});
   else if constexpr (AX || BX) go(Int<256>{}, Int<2>{}, Int<4>{});
-  else go(Int<256>{}, Int<4>{}, Int<2>{});
+  else go(Int<256>{}, Int<2>{}, Int<2>{});
   const int rc = check_launch("checkpointed_linear");
   if (rc != 0 || p.splits == 1) return rc;
   // (many runs: over several threads)

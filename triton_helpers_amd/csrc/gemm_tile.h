@@ -194,6 +194,7 @@ template <typename EL, int BM, int BN, int WM, int WN, bool AX = false, bool BX 
 struct Gemm {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16, ROWS_M = BM, WAVES_N = WN;
+  static constexpr int WAVES_SIMD = FM * FN > 32 ? 1 : 2;  // a wave of 128 x 128 takes all of a SIMD's registers
   typedef Side<AX, BM, WAVES> A;
   typedef Side<BX, BN, WAVES> B;
   static constexpr int SLOT = A::BYTES > B::BYTES ? A::BYTES : B::BYTES, SLOTS = 5;
@@ -282,45 +283,54 @@ struct Gemm {
     wait_and_meet<0>();  // nothing may still be on its way to LDS when it is used again, or at the workgroup's end
   }
 
-  // The sums in rows: body(m, v, ask(m)) for eight neighbouring columns from column() on, each row of the wave's part once, behind run().  They
-  // go through LDS, so that a row leaves in whole cache lines and the code behind them is one short loop (unrolled over the tiles it
-  // costs a small product more in instruction fetches than its sums).  ask() loads what a row's results go together with: for all rows of a pass at
-  // once, ahead of the pass before.
+  // The sums in rows, behind run(): pass(rows) once or twice, where rows(body) calls body(m, v, ask(m)) for eight neighbouring columns from column() on of each row of
+  // the pass.  They go through LDS, so that a row leaves in whole cache lines, and what the caller tells apart (types, activations) it tells apart behind
+  // them, not with the accumulators live in every branch.  ask() loads what a row's results go together with, four rows ahead of their use.
   static constexpr int LPR = 2 * FN;  // lanes to a row
   __device__ static __forceinline__ int column(const Tile& t) {
     return t.n * BN + (int)(threadIdx.x >> 6) % WN * (BN / WN) + (int)(threadIdx.x & 63) % LPR * 8;
   }
-  template <typename Acc, typename Ask, typename Body>
-  __device__ static __forceinline__ void each8(const Tile& t, char* lds, const Acc (&acc)[FM][FN], Ask&& ask, Body&& body) {
+  template <typename Acc, typename Ask, typename Pass>
+  __device__ static __forceinline__ void each8(const Tile& t, char* lds, const Acc (&acc)[FM][FN], Ask&& ask, Pass&& pass) {
     typedef typename std::remove_cv<typename std::remove_reference<decltype(acc[0][0][0])>::type>::type E;
     constexpr int LD = 16 * FN + 4, PASSES = 16 * FM * LD * 4 * WAVES <= LDS ? 1 : 2, ROWS = 16 * FM / PASSES, STRIDE = 64 / LPR;
     static_assert(ROWS * LD * 4 * WAVES <= LDS, "a strip for every wave");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m0 = t.m * BM + wave / WN * (BM / WM);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m0 = t.m * BM + wave / WN * (BM / WM) + lane / LPR;
     E* strip = (E*)lds + wave * (ROWS * LD);
-    constexpr int N = ROWS / STRIDE;  // rows of a lane and pass
-    decltype(ask(0)) with[2][N];
-    const auto ask_all = [&](int p) {
+    constexpr int GROUP = ROWS / STRIDE < 4 ? ROWS / STRIDE : 4;  // rows of a lane and turn of the loop
+    decltype(ask(0)) with[GROUP];
+    const auto ask_for = [&](int m) {
 #pragma unroll
-      for (int u = 0; u < N; ++u) with[p & 1][u] = ask(m0 + p * ROWS + lane / LPR + u * STRIDE);
+      for (int u = 0; u < GROUP; ++u) with[u] = ask(m + u * STRIDE);
     };
-    ask_all(0);
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
+    ask_for(m0);
+    const auto run_pass = [&](auto p_c) {
+      constexpr int p = decltype(p_c)::value;
 #pragma unroll
       for (int i = 0; i < FM / PASSES; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) *(Acc*)(strip + (16 * i + (lane & 15)) * LD + 16 * j + 4 * (lane >> 4)) = acc[p * (FM / PASSES) + i][j];
-      if (p + 1 < PASSES) ask_all(p + 1);
+      pass([&](auto&& body) {
+#pragma unroll 1
+        for (int r = 0; r < ROWS; r += GROUP * STRIDE) {
+          const int m = m0 + p * ROWS + r;
+          decltype(ask(0)) now[GROUP];
 #pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const int r = lane / LPR + u * STRIDE;
-        E v[8];
-        const E* from = strip + r * LD + lane % LPR * 8;
-        *(Acc*)v = *(const Acc*)from;
-        *(Acc*)(v + 4) = *(const Acc*)(from + 4);
-        body(m0 + p * ROWS + r, v, with[p & 1][u]);
-      }
-    }
+          for (int u = 0; u < GROUP; ++u) now[u] = with[u];
+          ask_for(m + GROUP * STRIDE);  // (behind a tile's end: masked as rows that are not there)
+#pragma unroll
+          for (int u = 0; u < GROUP; ++u) {
+            E v[8];
+            const E* from = strip + (lane / LPR + r + u * STRIDE) * LD + lane % LPR * 8;
+            *(Acc*)v = *(const Acc*)from;
+            *(Acc*)(v + 4) = *(const Acc*)(from + 4);
+            body(m + u * STRIDE, v, now[u]);
+          }
+        }
+      });
+    };
+    run_pass(Int<0>{});
+    if constexpr (PASSES == 2) run_pass(Int<1>{});
   }
 
   static constexpr int PER_ROW = (A::LOADS + FM - 1) / FM > (B::LOADS + FM - 1) / FM ? (A::LOADS + FM - 1) / FM : (B::LOADS + FM - 1) / FM;

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * W) void int8_few_rows_k(FewRows a) {
 
 // ---- tiles --------------------------------------------------------------------------------------
 template <typename G>
-__global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogue e, int* slots) {
+__global__ __launch_bounds__(G::THREADS, G::WAVES_SIMD) void int8_tile_k(GemmArgs g, Epilogue e, int* slots) {
   __shared__ __attribute__((aligned(1024))) char lds[G::LDS];
   i32x4_t acc[G::FM][G::FN] = {};
   const Tile t = tile_of(g, blockIdx.x);
@@ -160,15 +160,19 @@ __global__ __launch_bounds__(G::THREADS, 2) void int8_tile_k(GemmArgs g, Epilogu
   if (slots != nullptr) {  // [split][m][n rounded up to 8]
     const int64_t ld = (g.n + 7) / 8 * 8;
     int* o = slots + (int64_t)t.split * g.m * ld + n;
-    G::each8(t, lds, acc, [](int) { return 0; }, [&](int m, const int (&v)[8], int) {
-      if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+    G::each8(t, lds, acc, [](int) { return 0; }, [&](auto&& rows) {
+      rows([&](int m, const int (&v)[8], int) {
+        if (m < g.m && n < g.n) __builtin_memcpy(__builtin_assume_aligned(o + (int64_t)m * ld, 16), v, 32);
+      });
     });
     return;
   }
   const Columns columns(e, n);
-  with_epilogue(e, [&](auto act_c, auto y_c) {
-    G::each8(t, lds, acc, [&](int m) { return e.s[m < g.m ? m : g.m - 1]; }, [&](int m, const int (&v)[8], float s) {
-      if (m < g.m && n < g.n) put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, v, s, columns);
+  G::each8(t, lds, acc, [&](int m) { return e.s[m < g.m ? m : g.m - 1]; }, [&](auto&& rows) {
+    with_epilogue(e, [&](auto act_c, auto y_c) {
+      rows([&](int m, const int (&v)[8], float s) {
+        if (m < g.m && n < g.n) put8<decltype(act_c)::value, decltype(y_c)>(e, m, n, v, s, columns);
+      });
     });
   });
 }
@@ -297,6 +301,7 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   }
   const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)k, 0, 0, p.tile.splits, p.tile.split_steps};
   int* slots = p.tile.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
+  // (four waves of 128 x 128 in 8 bits: 1020 us instead of 820, the compiler moves accumulators about inside the loop)
   const int rc = p.tile.bm == 256 ? tile_launch<256, 256, 4, 2>(g, e, slots, s) : tile_launch<128, 128, 2, 2>(g, e, slots, s);
   if (rc != 0 || slots == nullptr) return rc;
   hipLaunchKernelGGL(int8_sum_k, dim3((unsigned)((rows * ((n + 7) / 8) + 255) / 256)), dim3(256), 0, s, slots, p.tile.splits, e);
