@@ -85,6 +85,14 @@ def test_large(m, n, k, dtype, name):
 
 
 @pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,n,k", [(8000, 1500, 5000), (8001, 5001, 1500), (1180, 3784, 7299), (13577, 5960, 301), (12022, 3075, 1550)])
+def test_large_tiles_with_split_sums(m, n, k, dtype):
+    """Tiles that fill the chip unevenly: the sum of one of the products is cut into a few runs."""
+    args = whole(m, n, k, dtype, seed=n)
+    check_exact(step(*args, "relu"), exact(*args, "relu"))
+
+
+@pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("m", [2047, 2048, 2049, 12287, 12288, 12319, 40001])
 @pytest.mark.parametrize("n,k", [(8, 8), (64, 128), (128, 64), (136, 120), (120, 136), (256, 256), (248, 32), (16, 256), (128, 128), (264, 256), (256, 264)])
 def test_many_rows_few_channels(m, n, k, dtype):

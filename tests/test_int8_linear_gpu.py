@@ -72,6 +72,12 @@ def test_large(m, n, k, dtype):
     check(int8_linear(q, s, w, t, b, dtype=dtype), q, s, w, t, b)
 
 
+@pytest.mark.parametrize("m,n,k", [(1272, 5069, 12532), (1500, 5000, 16000), (9584, 880, 13746)])
+def test_large_tiles_with_split_sums(m, n, k):
+    q, s, w, t, b = case(m, n, k, torch.float32, seed=k)
+    check(int8_linear(q, s, w, t, b, "silu"), q, s, w, t, b, "silu")
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(7, 90, 300), (150, 90, 300), (150, 136, 6000)])

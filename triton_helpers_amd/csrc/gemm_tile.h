@@ -422,8 +422,11 @@ inline int64_t round_up(int64_t v, int64_t unit) { return (v + unit - 1) / unit 
 // whether rows of `bytes` with `ld` bytes between them can be read as they are; 256 of them stay inside 31 bits
 inline bool rows_fit(const void* p, int64_t ld, int64_t bytes) { return bytes % 16 == 0 && ld % 16 == 0 && (uintptr_t)p % 16 == 0 && ld < (1 << 22); }
 
-// Tiles of 256 x 256, one to a compute unit, or of 128 x 128, two to one (two take 0.57 of the time of a large one, one alone 0.33): what needs
-// less for all of them.  Where even the small ones leave compute units idle the summed dimension is cut into runs of steps.
+// Tiles of 256 x 256, one to a compute unit, or of 128 x 128, two to one (two take 0.7 of the time of a large one, one alone 0.4), and the summed dimension in
+// `splits` runs of steps: what takes the least time for all of them.  us: 1.6 for a step of 256 x 256 on all units, 8 (small tiles 3) for a round's way in and out, and for
+// partial sums another launch, written and read at 4.5 TB/s.  What it chooses against the choice by tiles alone, bf16, us: dW of 4426 x 1907 over 29941 rows (five
+// runs of large tiles, one of small) 550 / 951, of 1600 x 3264 over 26317 332 / 497; 1180 x 3784 x 7299 76 / 85; without runs 29941 x 1907 x 4426 crosswise 461 / 619;
+// never more than the 3 % that runs differ by over 39 such shapes.
 struct TilePlan {
   int bm, splits, split_steps;
   int64_t slot_bytes;
@@ -431,18 +434,26 @@ struct TilePlan {
 inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
   constexpr int64_t CUS = 256;
   TilePlan p{};
-  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128), last = small % (2 * CUS);
-  const double cost_big = (double)((big + CUS - 1) / CUS), cost_small = 0.57 * (double)(small / (2 * CUS)) + (last == 0 ? 0.0 : last <= CUS ? 0.33 : 0.57);
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
   const int64_t steps = (kbytes + STEP - 1) / STEP;
-  p.bm = cost_big <= cost_small ? 256 : 128;
+  const auto sums = [&](int64_t s) { return s == 1 ? 0.0 : 2.5 + (double)(s * m * n) * 8.0 / 4.5e6; };
   int64_t splits = 1;
-  if (p.bm == 128 && small <= CUS) {
-    // us: 0.85 for a step (what memory takes to answer; 2^18 rows into 256 x 256 took 142 instead of 62 with 27 runs instead of 128), and for
-    // partial sums another launch, written and read at 4.5 TB/s
-    double best = 1e30;
+  double best = 1e30;
+  if (small <= CUS) {
+    // few tiles: 0.85 for a step, what memory takes to answer (2^18 rows into 256 x 256 took 142 instead of 62 with 27 runs instead of 128)
+    p.bm = 128;
     for (int64_t s = 1; s == 1 || (s * small <= 2 * CUS && s * 2 <= steps); s = s < 8 ? s + 1 : s * 5 / 4) {
-      const double cost = 0.85 * (double)((steps + s - 1) / s) + (s == 1 ? 0.0 : 2.5 + (double)(s * m * n) * 8.0 / 4.5e6);
+      const double cost = 0.85 * (double)((steps + s - 1) / s) + sums(s);
       if (cost < best) best = cost, splits = s;
+    }
+  } else {
+    for (int64_t s = 1; s == 1 || (s <= 8 && s * 8 <= steps); ++s) {
+      const int64_t full = s * small / (2 * CUS), last = s * small % (2 * CUS), rounds = (s * big + CUS - 1) / CUS;
+      const double each = 1.6 * (double)((steps + s - 1) / s), more = sums(s);
+      const double cost_big = (each + 8.0) * (double)rounds + more;
+      const double cost_small = (0.7 * each + 3.0) * (double)full + (last == 0 ? 0.0 : (last <= CUS ? 0.4 : 0.7) * each + 3.0) + more;
+      if (cost_big < best) best = cost_big, splits = s, p.bm = 256;
+      if (cost_small < best) best = cost_small, splits = s, p.bm = 128;
     }
   }
   p.split_steps = (int)((steps + splits - 1) / splits);
