@@ -160,13 +160,6 @@ __global__ __launch_bounds__(256) void keep_sum_k(const float* slots, int splits
 // What the backward's products read and the caller does not have: copies of dy and W on 16-byte boundaries, and act(s q) in 16 bits, each with rows
 // filled up with zeros to whole 16-byte pieces.  Streams, 16 bytes a thread and store; one launch for all of them (of what a small layer's step takes,
 // launches are the most).
-struct Copy {
-  const char* from;
-  int64_t ld, rows;
-  char* to;
-  int bytes;
-  int64_t blocks;  // none: nothing to copy
-};
 struct Prepare {
   Copy copy[2];
   const int8_t* q;
@@ -181,8 +174,7 @@ __global__ __launch_bounds__(256) void prepare_k(Prepare a) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (block < a.copy[c].blocks) {
-      const Copy& m = a.copy[c];
-      copy_rows<J>(block, m.from, m.ld, m.bytes, m.to, m.rows);
+      copy_rows<J>(block, a.copy[c]);
       return;
     }
     block -= a.copy[c].blocks;
@@ -356,7 +348,7 @@ int fwd(const KeepFwd& p, const void* x, int64_t xs, const void* w, int64_t ws, 
   if (q != nullptr || p.h_bytes > 0)
     if (const int rc = nf_quantize_rows(x, xs, T::code, q, scale, p.h_bytes > 0 ? h : nullptr, p.ldh, act, rows, k, stream)) return rc;
   if (p.w_bytes > 0)
-    if (const int rc = pack_rows((const char*)w, ws * 2, k * 2, packed, n, s)) return rc;
+    if (const int rc = pack_rows({w, ws * 2, n, k * 2, packed}, {}, s)) return rc;
   const GemmArgs g{p.h_bytes > 0 ? h : (const char*)x, p.w_bytes > 0 ? packed : (const char*)w, (p.h_bytes > 0 ? p.ldh : xs) * 2,
                    (p.w_bytes > 0 ? p.ldh : ws) * 2, (int)rows, (int)n, (int)k * 2, 0, 0, 0, 0};
   const Out e{y, ys, bias, bias_dt, NF_ACT_NONE, nullptr, nullptr, (int)rows, (int)n, T::code, nullptr, nullptr, 0};
@@ -384,7 +376,7 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
   int64_t blocks = 0;
   const int each = cut_pieces((p.dy_bytes + p.w_bytes + p.h_bytes) / 16);
   const auto copy = [&](int i, const void* from, int64_t ld, int64_t count, int64_t width, char* to) {
-    make.copy[i] = {(const char*)from, ld * 2, count, to, (int)width * 2, cut_blocks(count * ((width + 7) / 8), each)};
+    make.copy[i] = copy_of(from, ld * 2, count, width * 2, to, each);
     blocks += make.copy[i].blocks;
   };
   if (p.dy_bytes > 0) copy(0, dy, dys, rows, n, packed_dy);

@@ -393,22 +393,29 @@ inline int cut_pieces(int64_t pieces) { return pieces < (1 << 19) ? 1 : 4; }
 inline int64_t cut_blocks(int64_t pieces, int each) { return (pieces + 256 * each - 1) / (256 * each); }
 
 __device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
-// a workgroup's part of rows copied to 16-byte boundaries and filled up with zeros, a piece of 16 bytes
+// rows copied to 16-byte boundaries and filled up with zeros to whole pieces of 16 bytes; a workgroup's part of them
+struct Copy {
+  const char* from;
+  int64_t ld, rows;  // ld: bytes
+  char* to;
+  int bytes;       // of a row
+  int64_t blocks;  // none: nothing to copy
+};
 template <int J>
-__device__ __forceinline__ void copy_rows(int64_t block, const char* from, int64_t ld, int bytes, char* to, int64_t rows) {
-  const Cut<J> cut(block, (bytes + 15) / 16);
+__device__ __forceinline__ void copy_rows(int64_t block, const Copy& a) {
+  const Cut<J> cut(block, (a.bytes + 15) / 16);
   i32x4_t v[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     int piece;
     const int64_t row = cut.row(j, &piece);
-    if (row < rows) v[j] = load16(from + row * ld, piece * 16, bytes);
+    if (row < a.rows) v[j] = load16(a.from + row * a.ld, piece * 16, a.bytes);
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     int piece;
     const int64_t row = cut.row(j, &piece);
-    if (row < rows) *(i32x4_t*)(to + (row * cut.each + piece) * 16) = v[j];
+    if (row < a.rows) *(i32x4_t*)(a.to + (row * cut.each + piece) * 16) = v[j];
   }
 }
 
@@ -465,7 +472,15 @@ inline TilePlan tile_plan(int64_t m, int64_t n, int64_t kbytes) {
 inline bool tiles_fit(const TilePlan& p, int64_t m, int64_t n) {
   return (double)((m + p.bm - 1) / p.bm) * (double)((n + p.bm - 1) / p.bm) * p.splits * (2 * p.bm) < 4294967296.0;
 }
-// copies rows to 16-byte boundaries, filled up with zeros to whole 16-byte pieces (int8_linear.hip)
-int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s);
+inline Copy copy_of(const void* from, int64_t ld, int64_t rows, int64_t bytes, char* to, int each) {
+  return {(const char*)from, ld, rows, to, (int)bytes, cut_blocks(rows * ((bytes + 15) / 16), each)};
+}
+// copies of one or two operands' rows in one launch (int8_linear.hip)
+struct Pack {
+  const void* from;
+  int64_t ld, rows, bytes;
+  char* to;  // NULL: nothing to copy
+};
+int pack_rows(const Pack& a, const Pack& b, hipStream_t s);
 
 }  // namespace nf

@@ -194,14 +194,20 @@ __global__ __launch_bounds__(256) void int8_sum_k(const int* slots, int splits, 
 }
 
 template <int J>
-__global__ __launch_bounds__(256) void pack_rows_k(const char* from, int64_t ld, int bytes, char* to, int64_t rows) {
-  copy_rows<J>(block_number(), from, ld, bytes, to, rows);
+__global__ __launch_bounds__(256) void pack_rows_k(Copy a, Copy b) {
+  const int64_t block = block_number();
+  if (block < a.blocks) copy_rows<J>(block, a);
+  else if (block - a.blocks < b.blocks) copy_rows<J>(block - a.blocks, b);
 }
 
-int pack_rows(const char* from, int64_t ld, int64_t bytes, char* to, int64_t rows, hipStream_t s) {
-  const int64_t pieces = (bytes + 15) / 16;
-  if (cut_pieces(rows * pieces) == 1) hipLaunchKernelGGL((pack_rows_k<1>), grid_of(cut_blocks(rows * pieces, 1)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
-  else hipLaunchKernelGGL((pack_rows_k<4>), grid_of(cut_blocks(rows * pieces, 4)), dim3(256), 0, s, from, ld, (int)bytes, to, rows);
+int pack_rows(const Pack& a, const Pack& b, hipStream_t s) {
+  const auto pieces = [](const Pack& p) { return p.to == nullptr ? 0 : p.rows * ((p.bytes + 15) / 16); };
+  const int each = cut_pieces(pieces(a) + pieces(b));
+  const auto copy = [&](const Pack& p) { return p.to == nullptr ? Copy{} : copy_of(p.from, p.ld, p.rows, p.bytes, p.to, each); };
+  const Copy ca = copy(a), cb = copy(b);
+  const dim3 grid = grid_of(ca.blocks + cb.blocks);
+  if (each == 1) hipLaunchKernelGGL((pack_rows_k<1>), grid, dim3(256), 0, s, ca, cb);
+  else hipLaunchKernelGGL((pack_rows_k<4>), grid, dim3(256), 0, s, ca, cb);
   return check_launch("pack_rows");
 }
 
@@ -289,15 +295,11 @@ extern "C" int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* sc
   char* ws = (char*)workspace;
   const char *a = (const char*)q, *b = (const char*)w;
   int64_t lda = q_stride, ldb = w_stride;
-  if (p.q_bytes > 0) {
-    if (const int rc = pack_rows(a, lda, k, ws, rows, s)) return rc;
-    a = ws;
-    lda = round_up(k, 16);
-  }
-  if (p.w_bytes > 0) {
-    if (const int rc = pack_rows(b, ldb, k, ws + p.q_bytes, n, s)) return rc;
-    b = ws + p.q_bytes;
-    ldb = round_up(k, 16);
+  if (p.q_bytes > 0) a = ws, lda = round_up(k, 16);
+  if (p.w_bytes > 0) b = ws + p.q_bytes, ldb = round_up(k, 16);
+  if (p.q_bytes + p.w_bytes > 0) {
+    const Pack of_q{q, q_stride, rows, k, p.q_bytes > 0 ? ws : nullptr}, of_w{w, w_stride, n, k, p.w_bytes > 0 ? ws + p.q_bytes : nullptr};
+    if (const int rc = pack_rows(of_q, of_w, s)) return rc;
   }
   const GemmArgs g{a, b, lda, ldb, (int)rows, (int)n, (int)k, 0, 0, p.tile.splits, p.tile.split_steps};
   int* slots = p.tile.splits > 1 ? (int*)(ws + p.q_bytes + p.w_bytes) : nullptr;
