@@ -5,18 +5,17 @@
 
 namespace {
 
-// An eager graph of a leaf that is still alive holds the node that adds up the leaf's gradient, on the stream that it was built on.  A backward that
-// is captured would end there: a stream outside of the capture has to wait for the captured one, and torch ends the process.
-// Refused in the forward, while nothing has happened yet.
+// An eager graph of a leaf that is still alive holds the node that adds up the leaf's gradient, on the stream that it was built on.  Where that is the
+// default stream, which cannot take part in a capture, a captured backward would end there: it has to wait for the captured stream, and torch ends the
+// process.  Refused in the forward, while nothing has happened yet.  (Any other stream joins the capture and is joined again.)
 void refuse_eager_graph(const Tensor& t) {
   if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
   if (node == nullptr || node->num_inputs() == 0) return;
-  const auto here = c10::hip::getCurrentHIPStream(t.device().index());
-  if (node->input_metadata(0).stream().id() == here.id() ||
+  if (node->input_metadata(0).stream().id() != c10::hip::getDefaultHIPStream(t.device().index()).id() ||
       c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
     return;
-  TORCH_CHECK(false, "a graph that was built outside of this capture still holds one of the leaves: delete what it computed (outputs, losses) before capturing a "
+  TORCH_CHECK(false, "a graph that was built outside of this capture, on the default stream, still holds one of the leaves: delete what it computed (outputs, losses) before capturing a "
                      "step that takes gradients");
 }
 
