@@ -345,9 +345,12 @@ int fwd(const KeepFwd& p, const void* x, int64_t xs, const void* w, int64_t ws, 
   float* slots = (float*)(packed + p.w_bytes);
   hipStream_t s = (hipStream_t)stream;
   if (p.narrow) return narrow_fwd({x, w, bias, y, q, scale, xs, ws, ys, rows, (int)n, (int)k, bias_dt, act}, T::code, s);
-  if (q != nullptr || p.h_bytes > 0)
-    if (const int rc = nf_quantize_rows(x, xs, T::code, q, scale, p.h_bytes > 0 ? h : nullptr, p.ldh, act, rows, k, stream)) return rc;
-  if (p.w_bytes > 0)
+  const bool beside = p.w_bytes > 0 && p.h_bytes > 0 && k <= MOST_BESIDE && cut_pieces(p.w_bytes / 16) == 1;
+  if (q != nullptr || p.h_bytes > 0) {
+    const Copy also = beside ? copy_of(w, ws * 2, n, k * 2, packed, 1) : Copy{};
+    if (const int rc = quantize_and_copy(x, xs, T::code, q, scale, p.h_bytes > 0 ? h : nullptr, p.ldh, act, rows, k, also, s)) return rc;
+  }
+  if (p.w_bytes > 0 && !beside)
     if (const int rc = pack_rows({w, ws * 2, n, k * 2, packed}, {}, s)) return rc;
   const GemmArgs g{p.h_bytes > 0 ? h : (const char*)x, p.w_bytes > 0 ? packed : (const char*)w, (p.h_bytes > 0 ? p.ldh : xs) * 2,
                    (p.w_bytes > 0 ? p.ldh : ws) * 2, (int)rows, (int)n, (int)k * 2, 0, 0, 0, 0};

@@ -482,5 +482,10 @@ struct Pack {
   char* to;  // NULL: nothing to copy
 };
 int pack_rows(const Pack& a, const Pack& b, hipStream_t s);
+// nf_quantize_rows on checked arguments; where h is asked for and rows hold at most MOST_BESIDE values, `also` (one piece a thread) is copied in the same launch
+// (quantize_rows.hip)
+constexpr int64_t MOST_BESIDE = 32768;
+int quantize_and_copy(const void* x, int64_t xs, int dtype, int8_t* q, float* scale, void* h, int64_t hs, int act, int64_t rows, int64_t width, const Copy& also,
+                      hipStream_t s);
 
 }  // namespace nf

@@ -3,7 +3,7 @@
 //
 // A stream over HBM: a row is read once and held in registers between its maximum and its rounding; rows above 32768 values are read twice.  Short rows
 // share a wave (2^18 x 256 57 us instead of 107).  16384 x 4096 bf16 with GELU: 61 us, 335 MB at 5.5 TB/s.
-#include "wide_common.h"
+#include "gemm_tile.h"
 
 namespace nf {
 
@@ -14,6 +14,8 @@ struct Quantize {
   void* h;  // NULL, or rows of x's type with `hs` values between them; values behind the row's end become zeros
   int64_t xs, hs, rows;
   int width;
+  Copy also;  // next to h: rows of another operand, by workgroups behind those of the rows (a launch less for a small layer)
+  unsigned row_blocks;
 };
 
 template <typename XT, int ACT>
@@ -28,6 +30,12 @@ __device__ __forceinline__ void put_act(const Quantize& a, int64_t row, int c, c
 template <typename XT, int T, int NV, int ACT, bool KEEP>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_k(Quantize a) {
   __shared__ uint32_t tops[16];
+  if constexpr (KEEP) {
+    if (blockIdx.x >= a.row_blocks) {
+      if (threadIdx.x < 256) copy_rows<1>(blockIdx.x - a.row_blocks, a.also);
+      return;
+    }
+  }
   const int t = threadIdx.x % T;
   const int64_t row = T < 256 ? (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T : blockIdx.x;
   if (row >= a.rows) return;  // up to T = 64: all threads of a row, which meet no barrier
@@ -87,11 +95,12 @@ __global__ __launch_bounds__(1024) void quantize_wide_k(Quantize a) {
 }
 
 template <typename XT, int ACT, bool KEEP>
-int quantize_launch_some(const Quantize& a, hipStream_t s) {
+int quantize_launch_some(Quantize a, hipStream_t s) {
   const auto go = [&](auto t_c, auto nv_c) {
     constexpr int T = decltype(t_c)::value, NV = decltype(nv_c)::value;
     const int64_t per = T < 256 ? 256 / T : 1;
-    hipLaunchKernelGGL((quantize_k<XT, T, NV, ACT, KEEP>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(T < 256 ? 256 : T), 0, s, a);
+    a.row_blocks = (unsigned)((a.rows + per - 1) / per);
+    hipLaunchKernelGGL((quantize_k<XT, T, NV, ACT, KEEP>), dim3(a.row_blocks + (unsigned)a.also.blocks), dim3(T < 256 ? 256 : T), 0, s, a);
   };
   // a few rows: as many threads to each as its values take
   if (a.rows <= 512 && a.width > 512 && a.width <= 2048) go(Int<256>{}, Int<1>{});
@@ -117,6 +126,7 @@ int quantize_launch(const Quantize& a, hipStream_t s) {
     part.x = (const X*)a.x + row * a.xs;
     if (a.q != nullptr) part.q = a.q + row * a.width, part.scale = a.scale + row;
     if (a.h != nullptr) part.h = (X*)a.h + row * a.hs;
+    if (row > 0) part.also.blocks = 0;
     if (const int rc = quantize_launch_some<XT, ACT, KEEP>(part, s)) return rc;
   }
   return 0;
@@ -134,6 +144,14 @@ int quantize_by_act(const Quantize& a, int act, hipStream_t s) {
   }
 }
 
+int quantize_and_copy(const void* x, int64_t xs, int dtype, int8_t* q, float* scale, void* h, int64_t hs, int act, int64_t rows, int64_t width, const Copy& also,
+                      hipStream_t s) {
+  const Quantize a{x, q, scale, h, xs, hs, rows, (int)width, also, 0};
+  if (dtype == NF_F32) return quantize_by_act<F32>(a, act, s);
+  if (dtype == NF_F16) return quantize_by_act<F16>(a, act, s);
+  return quantize_by_act<BF16>(a, act, s);
+}
+
 }  // namespace nf
 
 using namespace nf;
@@ -149,9 +167,5 @@ extern "C" int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, in
   if (rows == 0) return 0;
   NF_REQUIRE(x && (q ? scale != nullptr : h != nullptr), NF_EINVAL, "NULL pointer argument");
   NF_REQUIRE(rows == 1 || x_stride >= width, NF_EINVAL, "row stride below the width");
-  const Quantize a{x, q, scale, h, x_stride, h_stride, rows, (int)width};
-  hipStream_t s = (hipStream_t)stream;
-  if (x_dtype == NF_F32) return quantize_by_act<F32>(a, act, s);
-  if (x_dtype == NF_F16) return quantize_by_act<F16>(a, act, s);
-  return quantize_by_act<BF16>(a, act, s);
+  return quantize_and_copy(x, x_stride, x_dtype, q, scale, h, h_stride, act, rows, width, Copy{}, (hipStream_t)stream);
 }
