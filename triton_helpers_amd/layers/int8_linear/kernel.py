@@ -16,6 +16,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import Function
 
 from ... import _lib
 
@@ -32,23 +33,11 @@ def _no_grad(name: str, *tensors: Optional[Tensor]) -> None:
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
-def quantize_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
-    r"""The 8-bit form of the rows of ``x``, also that of a weight :math:`(N, K)`; for inference.
-
-    Shapes:
-        - x: :math:`(..., K)`, float32 / float16 / bfloat16, any row strides
-        - Output: ``(q, scale)``, int8 :math:`(..., K)` and float32 :math:`(...)`
-    """
-    out = _lib.native().quantize_rows(x)
-    if out is not None:
-        return out
+def _validate_rows(x: Tensor) -> None:
     assert x.ndim >= 1 and x.shape[-1] >= 1, "x must have a last dimension of at least one value"
     if x.dtype not in _TYPES:
         raise NotImplementedError(f"quantize_rows takes float16 / bfloat16 / float32 rows, got {x.dtype}")
     assert x.device.type == "cuda", "All tensors must be on a GPU device"
-    _no_grad("quantize_rows", x)
-    with torch.no_grad():
-        return _lib.native().quantize_rows_launch(x)
 
 
 def _validate(q: Tensor, scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], activation: str, dtype: torch.dtype) -> None:
@@ -70,6 +59,38 @@ def _validate(q: Tensor, scale: Tensor, w: Tensor, w_scale: Tensor, bias: Option
     assert q.device.type == "cuda", "All tensors must be on a GPU device"
 
 
+# The launches as autograd Functions, though they have no gradient: a traced function then holds the operator (the tracer would record the
+# allocation of the results and nothing of the launch), and tangents and transforms are refused.
+# A call of the traced function comes to ``forward`` alone, with whatever tensors it is given.
+class _quantize_rows(Function):
+    @staticmethod
+    def forward(ctx, x: Tensor) -> Tuple[Tensor, Tensor]:
+        _validate_rows(x)
+        return _lib.native().quantize_rows_launch(x)
+
+
+class _int8_linear(Function):
+    @staticmethod
+    def forward(ctx, q: Tensor, scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], activation: str, dtype: torch.dtype) -> Tensor:
+        _validate(q, scale, w, w_scale, bias, activation, dtype)
+        return _lib.native().int8_linear_launch(q, scale, w, w_scale, bias, _lib.NF_ACT[activation], _CODE[dtype])
+
+
+def quantize_rows(x: Tensor) -> Tuple[Tensor, Tensor]:
+    r"""The 8-bit form of the rows of ``x``, also that of a weight :math:`(N, K)`; for inference.
+
+    Shapes:
+        - x: :math:`(..., K)`, float32 / float16 / bfloat16, any row strides
+        - Output: ``(q, scale)``, int8 :math:`(..., K)` and float32 :math:`(...)`
+    """
+    out = _lib.native().quantize_rows(x)
+    if out is not None:
+        return out
+    _validate_rows(x)
+    _no_grad("quantize_rows", x)
+    return _quantize_rows.apply(x)
+
+
 def int8_linear(q: Tensor, scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = None, activation: str = "none",
                 dtype: torch.dtype = torch.bfloat16) -> Tensor:
     r"""Product of 8-bit rows with 8-bit weight rows; for inference.
@@ -88,5 +109,4 @@ def int8_linear(q: Tensor, scale: Tensor, w: Tensor, w_scale: Tensor, bias: Opti
         return y
     _validate(q, scale, w, w_scale, bias, activation, dtype)
     _no_grad("int8_linear", scale, w_scale, bias)
-    with torch.no_grad():
-        return _lib.native().int8_linear_launch(q, scale, w, w_scale, bias, _lib.NF_ACT[activation], code)
+    return _int8_linear.apply(q, scale, w, w_scale, bias, activation, dtype)

@@ -57,6 +57,18 @@ class _rms_norm(Function):
         return dx, dw, None, dr
 
 
+class _rms_norm_int8(Function):
+    """The launch as a Function, though it has no gradient: a traced function then holds the operator (the tracer would record the allocation of the
+    results and nothing of the launch), and tangents and transforms are refused.  A call of the traced function comes to ``forward`` alone, with
+    whatever tensors it is given."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Optional[Tensor], eps: float, residual: Optional[Tensor]) -> Tuple[Tensor, ...]:
+        _validate(x, weight, eps, residual)
+        q, scale, stream, _ = _lib.native().rms_norm_launch_forward(x, weight, float(eps), residual, True)
+        return (q, scale) if residual is None else (q, scale, stream)
+
+
 def rms_norm(x: Tensor, weight: Optional[Tensor], eps: float = 1e-6, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
     r"""Norm of the rows of ``x`` (of ``x + residual``); differentiable once in all tensors.
 
@@ -87,6 +99,4 @@ def rms_norm_int8(x: Tensor, weight: Optional[Tensor], eps: float = 1e-6, residu
     _validate(x, weight, eps, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_int8 has no gradient: call it under torch.no_grad(), or rms_norm where one is needed")
-    with torch.no_grad():
-        q, scale, stream, _ = _lib.native().rms_norm_launch_forward(x, weight, float(eps), residual, True)
-    return (q, scale) if residual is None else (q, scale, stream)
+    return _rms_norm_int8.apply(x, weight, eps, residual)
