@@ -117,3 +117,133 @@ def test_function_transforms_are_refused(name):
         torch.func.grad(lambda x: total(1.0, x, *args[1:]))(args[0])
     for a, b in zip(several(fn(*args)), want):
         assert torch.equal(a, b)
+
+
+def _functions(name):
+    """The operator on the native host path and as its Python Function."""
+    from triton_helpers_amd.layers.checkpointed_linear.kernel import _checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm.kernel import _rms_norm
+
+    if name == "rms_norm":
+        return [lambda x, w: rms_norm(x, w), lambda x, w: _rms_norm.apply(x, w, 1e-6, None)]
+    if name == "rms_norm residual":
+        return [lambda x, w, r: rms_norm(x, w, 1e-6, r)[0], lambda x, w, r: _rms_norm.apply(x, w, 1e-6, r)[0]]
+    return [lambda x, w, b: checkpointed_linear(x, w, b, "gelu"), lambda x, w, b: _checkpointed_linear.apply(x, w, b, "gelu")]
+
+
+REFUSED = "differentiable once"
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("name", TRAINED)
+def test_a_second_derivative_beside_a_first_is_refused(name, python):
+    """A penalty on a gradient next to an ordinary loss: the second derivative raises, whichever tensors the backward is asked for."""
+    fn = _functions(name)[python]
+    leaves = [t.requires_grad_() for t in operator(name)[1]]
+    rows = leaves[:1] if name != "rms_norm residual" else [leaves[0], leaves[2]]
+
+    def mixed(of, upstream=None):
+        y = fn(*leaves)
+        dy = torch.ones_like(y) if upstream is None else upstream
+        first = torch.autograd.grad(y, of, dy, retain_graph=True)
+        g = torch.autograd.grad(y, of, dy, create_graph=True)
+        for a, b in zip(first, g):
+            assert torch.equal(a, b.detach())
+        assert all(t.requires_grad for t in g)
+        return y.float().sum() + sum(t.float().square().sum() for t in g)
+
+    for of in (rows, leaves[1:2]):
+        with pytest.raises(RuntimeError, match=REFUSED):
+            mixed(of).backward()
+        asked = leaves if of is rows else rows  # (the weight's gradient does not depend on the weight)
+        for leaf in asked[:2]:
+            with pytest.raises(RuntimeError, match=REFUSED):
+                torch.autograd.grad(mixed(of), leaf)
+        y = fn(*leaves)
+        dy = torch.randn_like(y).requires_grad_()
+        with pytest.raises(RuntimeError, match=REFUSED):
+            torch.autograd.grad(mixed(of, dy), dy)
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_gradients_that_are_constant_need_no_second_derivative(python):
+    """Without an activation dx depends on the weight alone, and db on the upstream gradient: where these are constant nothing is lost, and nothing refused."""
+    from triton_helpers_amd.layers.checkpointed_linear.kernel import _checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm.kernel import _rms_norm
+
+    linear = (lambda x, w, b, name="none": _checkpointed_linear.apply(x, w, b, name)) if python else checkpointed_linear
+    norm = (lambda x, w, eps=1e-6, r=None: _rms_norm.apply(x, w, eps, r)) if python else rms_norm
+    x, w, b = operator("checkpointed_linear")[1]
+    x, b = x.requires_grad_(), b.requires_grad_()
+    y = linear(x, w, b)
+    g = torch.autograd.grad(y.float().sum(), (x, b), create_graph=True)
+    assert not any(t.requires_grad for t in g)
+    (y.float().sum() + sum(t.float().square().sum() for t in g)).backward()
+    assert torch.equal(x.grad, g[0]) and torch.equal(b.grad, g[1])
+    y = linear(x, w, b, "gelu")
+    g, = torch.autograd.grad(y.float().sum(), b, create_graph=True)
+    assert not g.requires_grad
+    # the weight's part in dx, with x fixed
+    w.requires_grad_()
+    g, = torch.autograd.grad(linear(x, w, b).float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match=REFUSED):
+        torch.autograd.grad(g.float().sum(), w)
+    # the new residual's own gradient goes to x and r as it is
+    x, w, r = (t.requires_grad_() for t in operator("rms_norm residual")[1])
+    stream = norm(x, w, 1e-6, r)[1]
+    g = torch.autograd.grad(stream.float().sum(), (x, r), create_graph=True)
+    assert not any(t.requires_grad for t in g) and all(torch.equal(t, torch.ones_like(t)) for t in g)
+    ds = torch.randn_like(stream).requires_grad_()
+    g = torch.autograd.grad(norm(x, w, 1e-6, r)[1], (x, r), ds, create_graph=True)
+    with pytest.raises(RuntimeError, match=REFUSED):
+        torch.autograd.grad(g[1].float().sum(), ds)
+
+
+def test_a_second_derivative_under_autocast_is_refused():
+    x, w, b = (t.float().requires_grad_() for t in operator("checkpointed_linear")[1])
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = checkpointed_linear(x, w, b, "silu")
+    g = torch.autograd.grad(y.float().sum(), (x, w), create_graph=True)
+    assert all(t.dtype == torch.float32 for t in g)
+    for t, leaf in ((g[0], w), (g[1], x)):
+        with pytest.raises(RuntimeError, match=REFUSED):
+            torch.autograd.grad(t.sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match=REFUSED):
+        (y.float().sum() + g[0].square().sum()).backward()
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_what_the_backward_reads_may_not_change(python):
+    """Rows and weights that are kept as they are: a change between forward and backward raises.  Kept 8-bit rows are the layer's own."""
+    from triton_helpers_amd.layers.checkpointed_linear.kernel import _checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm.kernel import _rms_norm
+
+    linear = (lambda x, w, b, name="none": _checkpointed_linear.apply(x, w, b, name)) if python else checkpointed_linear
+    norm = (lambda x, w, eps=1e-6, r=None: _rms_norm.apply(x, w, eps, r)) if python else rms_norm
+    x, w, r = (t.requires_grad_() for t in operator("rms_norm residual")[1])
+    rows, weight = x * 1.0, w * 1.0
+    for changed in (rows, weight):
+        y = norm(rows, weight)
+        with torch.no_grad():
+            changed.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.float().sum().backward()
+    y, stream = norm(x, w, 1e-6, r)
+    with torch.no_grad():
+        stream.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+    x, w, b = (t.requires_grad_() for t in operator("checkpointed_linear")[1])
+    weight = w * 1.0
+    y = linear(x * 1.0, weight, b, "gelu")
+    with torch.no_grad():
+        weight.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+    want = torch.autograd.grad(linear(x, w, b, "gelu").float().sum(), (x, w))
+    rows = x * 1.0
+    y = linear(rows, w, b, "gelu")
+    with torch.no_grad():
+        rows.zero_()
+    for a, c in zip(torch.autograd.grad(y.float().sum(), (x, w)), want):
+        assert torch.equal(a, c)

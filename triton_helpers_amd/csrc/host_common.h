@@ -17,6 +17,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -66,6 +68,28 @@ struct Rows {
       stride = hold.stride(0);
     }
     p = hold.data_ptr();
+  }
+};
+
+// The gradients that a kernel computed have no graph.  Where one is asked for (create_graph), each of them that depends on something which requires a gradient gets a
+// node that raises: a second derivative is refused instead of lost.  The node leads to what the gradient depends on, so that a backward for
+// these tensors alone comes to it, too.
+struct Once {
+  const char* name;
+  std::shared_ptr<torch::autograd::Node> node;  // whose backward runs (none: no graph is asked for); its edges are the forward's tensors in their order
+  explicit Once(const char* what) : name(what), node(at::GradMode::is_enabled() ? torch::autograd::get_current_node() : nullptr) {}
+  // `inputs`: the numbers of the forward's tensors that g depends on; `grads`: the upstream gradients
+  void mark(const Tensor& g, std::initializer_list<int> inputs, std::initializer_list<Tensor> grads) const {
+    if (node == nullptr || !g.defined()) return;
+    torch::autograd::edge_list edges;
+    for (const int i : inputs)
+      if ((uint32_t)i < node->num_outputs() && node->next_edge(i).is_valid()) edges.push_back(node->next_edge(i));
+    for (const Tensor& t : grads)
+      if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+    if (edges.empty()) return;
+    const std::shared_ptr<torch::autograd::Node> raises(
+        new torch::autograd::Error(std::string(name) + " is differentiable once: its gradients have no derivatives", std::move(edges)), torch::autograd::deleteNode);
+    torch::autograd::set_history(g, raises);
   }
 };
 

@@ -95,6 +95,19 @@ variable_list norm_backward(const Tensor& h, const Tensor& rstd, const Tensor& w
   return {dx, dw, dr};
 }
 
+// The forward's tensors are x, the weight where there is one, the residual.
+void norm_once(const variable_list& g, const Tensor& dy, const Tensor& ds, bool weight) {
+  const Once once("rms_norm");
+  if (!dy.defined()) {  // the new residual's gradient goes on as it is
+    once.mark(g[0], {}, {ds});
+    if (g[2].defined() && !g[2].is_same(g[0])) once.mark(g[2], {}, {ds});
+    return;
+  }
+  once.mark(g[0], {0, 1, 2}, {dy, ds});
+  if (weight) once.mark(g[1], {0, 2}, {dy});
+  if (g[2].defined() && !g[2].is_same(g[0])) once.mark(g[2], {0, 1, 2}, {dy, ds});
+}
+
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, std::optional<Tensor> w, std::optional<Tensor> r, double eps) {
     const bool two = r && x.is_leaf() && r->is_leaf() && x.requires_grad() && r->requires_grad();
@@ -117,6 +130,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const bool need_rows = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(weight ? 2 : 1));
     variable_list g = norm_backward(s[0], s[1], s[2], (at::ScalarType)ctx->saved_data["type"].toInt(), grads[0], residual ? grads[1] : Tensor(), residual,
                                     need_rows, need_w, ctx->saved_data["two"].toBool());
+    norm_once(g, grads[0], residual ? grads[1] : Tensor(), weight);
     return {g[0], g[1], g[2], Tensor()};
   }
 };
@@ -204,6 +218,7 @@ PyObject* rms_norm_launch_backward(PyObject*, PyObject* const* a, Py_ssize_t n) 
     pybind11::gil_scoped_release release;
     const at::AutoDispatchBelowADInplaceOrView below;
     g = norm_backward(h, rstd, w, like.scalar_type(), dy, ds, residual, need_rows, need_w, residual);
+    norm_once(g, dy, ds, w.defined());
   }
   return wrap_list(g);
   END_HANDLE_TH_ERRORS
@@ -395,6 +410,15 @@ variable_list keep_backward(const Tensor& q, const Tensor& scale, const Tensor& 
   return {dx, dw, db};
 }
 
+// The forward's tensors are x, w, b.
+void keep_once(const variable_list& g, const Tensor& dy, int act) {
+  const Once once("checkpointed_linear");
+  if (act == NF_ACT_NONE) once.mark(g[0], {1}, {dy});
+  else once.mark(g[0], {0, 1}, {dy});
+  once.mark(g[1], {0}, {dy});
+  once.mark(g[2], {}, {dy});
+}
+
 struct LinearKeep : torch::autograd::Function<LinearKeep> {
   // cast: the type that autocast asks for, or the tensors' own
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, std::optional<Tensor> b, int64_t act, int64_t cast) {
@@ -413,9 +437,11 @@ struct LinearKeep : torch::autograd::Function<LinearKeep> {
     const variable_list s = ctx->get_saved_variables();
     const at::AutoDispatchBelowADInplaceOrView below;
     const int64_t bias = ctx->saved_data["bias"].toInt();
-    variable_list g = keep_backward(s[0], s[1], s[2], (int)ctx->saved_data["act"].toInt(), grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+    const int act = (int)ctx->saved_data["act"].toInt();
+    variable_list g = keep_backward(s[0], s[1], s[2], act, grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                     bias >= 0 && ctx->needs_input_grad(2), ctx->saved_data["float_dw"].toBool(),
                                     bias >= 0 ? (at::ScalarType)bias : at::kFloat);
+    keep_once(g, grads[0], act);
     g.resize(5);
     return g;
   }
@@ -479,6 +505,7 @@ PyObject* checkpointed_linear_launch_backward(PyObject*, PyObject* const* a, Py_
     pybind11::gil_scoped_release release;
     const at::AutoDispatchBelowADInplaceOrView below;
     r = keep_backward(q, scale, w, (int)act, dy, dx, dw, db, wide, bt == NF_F32 ? at::kFloat : bt == NF_F16 ? at::kHalf : at::kBFloat16);
+    keep_once(r, dy, (int)act);
   }
   return wrap_list(r);
   END_HANDLE_TH_ERRORS

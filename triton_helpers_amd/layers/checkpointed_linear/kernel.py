@@ -23,7 +23,6 @@ from typing import Optional
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ... import _lib
 
@@ -67,7 +66,6 @@ class _checkpointed_linear(Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy: Tensor):
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
         dx, dw, db = _lib.native().checkpointed_linear_launch_backward(

@@ -15,7 +15,6 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ... import _lib
 
@@ -49,7 +48,6 @@ class _rms_norm(Function):
         return y if residual is None else (y, stream)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy: Optional[Tensor], d_residual: Optional[Tensor] = None):
         h, rstd, weight = ctx.saved_tensors
         need_x, need_w, _, need_r = ctx.needs_input_grad
