@@ -160,11 +160,11 @@ __device__ __forceinline__ void store8_q(int8_t* p, int n, const float (&v)[8], 
       if (i < n) p[i] = (int8_t)(q[i / 4] >> (i % 4 * 8));
   }
 }
-// ... and back: s q.  (A byte less 128 as one multiplication and addition: 128 s is exact, so is nothing rounded but the result.)
+// ... and back: s q.  (A byte less 128 is exact, so nothing is rounded but the result.  As one multiplication and addition, s byte - 128 s, a row with
+// the largest bfloat16 values would have no finite 128 s.)
 __device__ __forceinline__ void kept8(const int (&q)[2], float s, float (&v)[8]) {
-  const float shift = -128.0f * s;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fmaf((float)(uint8_t)(((uint32_t)q[i / 4] ^ 0x80808080u) >> (i % 4 * 8)), s, shift);
+  for (int i = 0; i < 8; ++i) v[i] = s * ((float)(uint8_t)(((uint32_t)q[i / 4] ^ 0x80808080u) >> (i % 4 * 8)) - 128.0f);
 }
 // the largest magnitude of eight 16-bit values, in their type's bits
 __device__ __forceinline__ uint16_t largest16(const uint32_t (&v)[4]) {
