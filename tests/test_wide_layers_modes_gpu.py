@@ -247,3 +247,67 @@ def test_what_the_backward_reads_may_not_change(python):
         rows.zero_()
     for a, c in zip(torch.autograd.grad(y.float().sum(), (x, w)), want):
         assert torch.equal(a, c)
+
+
+def _transposed(t):
+    return t.t().contiguous().t() if t.dim() == 2 else torch.stack([t, t + 1], -1)[..., 0]
+
+
+def _shifted(t):
+    return torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("hook", [_transposed, _shifted, lambda t: t.cpu().cuda(), None])
+@pytest.mark.parametrize("m", [300, 4096])
+def test_saved_tensors_in_other_places(m, hook, python):
+    """What a saved-tensor hook hands back may have other strides and lie off 16-byte boundaries.
+
+    Weights off 16-byte boundaries go to other kernels, which add up dW's products in another order: both float32 sums of m products are off by at
+    most (m + 4) 2^-24 of the sum of their magnitudes, which is at most |dy|^T (|x| + a / 127) as |gelu(z)| <= |z| and the 8-bit rows are at most half a
+    step, a / 254, and a rounding off; each is rounded once, by half a step."""
+    from triton_helpers_amd.layers.checkpointed_linear.kernel import _checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm.kernel import _rms_norm
+
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x, w, dy = (torch.randn(*s, generator=g, device=DEV).bfloat16() for s in ((m, 64), (64, 64), (m, 64)))
+    v = torch.randn(64, generator=g, device=DEV)
+
+    def step(saved):
+        leaves = [t.clone().requires_grad_() for t in (x, w, v)]
+        xl, wl, vl = leaves
+        with saved:
+            y = _checkpointed_linear.apply(xl, wl, None, "gelu") if python else checkpointed_linear(xl, wl, None, "gelu")
+            u = _rms_norm.apply(xl, vl, 1e-6, None) if python else rms_norm(xl, vl)
+            z = (_rms_norm.apply(xl, vl, 1e-6, xl * 2) if python else rms_norm(xl, vl, 1e-6, xl * 2))[0]
+        torch.autograd.backward((y, u, z), (dy, dy, dy))
+        return [t.grad for t in leaves]
+
+    want = step(torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t))
+    got = step(torch.autograd.graph.save_on_cpu() if hook is None else torch.autograd.graph.saved_tensors_hooks(lambda t: t, hook))
+    if hook is _shifted:
+        h = x.double().abs() + x.double().abs().amax(-1, keepdim=True) / 127
+        bound = 2 * (m + 4) * 2.0**-24 * (dy.double().abs().t() @ h) + 2 * 2.0**-8 * torch.maximum(got[1].double().abs(), want[1].double().abs())
+        assert ((got.pop(1).double() - want.pop(1).double()).abs() <= bound).all()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", TRAINED)
+def test_checkpointed_gradients(name):
+    """A saved-tensor hook that recomputes (non-reentrant checkpointing) runs with autograd on inside the operator's backward."""
+    from torch.utils.checkpoint import checkpoint
+
+    fn, args = operator(name)
+
+    def region(*a):  # the operator's tensors come out of a differentiable operation inside the checkpointed region
+        return several(fn(*(t * 1.5 for t in a)))
+
+    got = []
+    for through in (region, lambda *a: checkpoint(region, *a, use_reentrant=False)):
+        leaves = [t.detach().clone().requires_grad_() for t in args]
+        out = through(*leaves)
+        torch.autograd.backward(out, [torch.ones_like(t) for t in out])
+        got.append([*(t.detach() for t in out), *(t.grad for t in leaves)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

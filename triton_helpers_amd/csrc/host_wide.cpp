@@ -68,7 +68,7 @@ NormOut norm_forward(const Norm& m, bool eight, bool keep) {
 variable_list norm_backward(const Tensor& h, const Tensor& rstd, const Tensor& weight, at::ScalarType xt, Tensor dy, Tensor ds, bool residual,
                             bool need_rows, bool need_w, bool two) {
   const c10::DeviceGuard guard(h.device());
-  const int64_t width = h.size(-1);
+  const int64_t width = h.size(-1);  // (h and the factors may come back from a saved-tensor hook in any layout)
   const auto ht = h.scalar_type();
   if (!dy.defined()) dy = at::zeros(h.sizes(), h.options().dtype(xt));
   if (dy.scalar_type() != xt) dy = dy.to(xt);
@@ -76,7 +76,7 @@ variable_list norm_backward(const Tensor& h, const Tensor& rstd, const Tensor& w
   const Rows rh(h, width), rd(dy, width);
   std::optional<Rows> rs;
   if (ds.defined()) rs.emplace(ds, width);
-  const Tensor w = contiguous(weight);
+  const Tensor w = contiguous(weight), factors = contiguous(rstd);
   Tensor dx, dr, dw;
   if (need_rows) {
     dx = at::empty(h.sizes(), h.options().dtype(xt));
@@ -88,7 +88,7 @@ variable_list norm_backward(const Tensor& h, const Tensor& rstd, const Tensor& w
     const int64_t bytes = need_w ? nf_rms_norm_bwd_workspace_bytes(rh.n, width) : 0;
     const Tensor ws = scratch(bytes, h);
     check(nf_rms_norm_bwd(rd.p, rd.stride, code_of(xt), rs ? rs->p : nullptr, rs ? rs->stride : width, rh.p, rh.stride, code_of(ht),
-                          rstd.data_ptr<float>(), ptr(w), w.defined() ? code_of(w.scalar_type()) : NF_F32, ptr(dx),
+                          factors.data_ptr<float>(), ptr(w), w.defined() ? code_of(w.scalar_type()) : NF_F32, ptr(dx),
                           dr.defined() && !dr.is_same(dx) ? dr.data_ptr() : nullptr, ptr(dw), rh.n, width, ptr(ws), bytes, stream_of(h)),
           "nf_rms_norm_bwd");
   }
@@ -385,11 +385,15 @@ variable_list keep_forward(const Keep& m, bool keep) {
 }
 
 // (dx, dw, db); dw in float32 where `float_dw`, db of type `bt`
-variable_list keep_backward(const Tensor& q, const Tensor& scale, const Tensor& weight, int act, Tensor dy, bool need_dx, bool need_dw, bool need_db,
+variable_list keep_backward(Tensor q, Tensor scale, const Tensor& weight, int act, Tensor dy, bool need_dx, bool need_dw, bool need_db,
                             bool float_dw, at::ScalarType bt) {
   const c10::DeviceGuard guard(weight.device());
   const int64_t n = weight.size(0), k = weight.size(1);
   if (dy.scalar_type() != weight.scalar_type()) dy = dy.to(weight.scalar_type());
+  // (what was kept may come back from a saved-tensor hook in any layout)
+  q = contiguous(q);
+  scale = contiguous(scale);
+  if (q.defined() && (uintptr_t)q.data_ptr() % 16 != 0) q = q.clone();
   const Rows g(dy, n), w(weight, k);
   Tensor dx, dw, db;
   c10::SmallVector<int64_t, 5> shape(dy.sizes().begin(), dy.sizes().end());
