@@ -311,3 +311,36 @@ def test_checkpointed_gradients(name):
         got.append([*(t.detach() for t in out), *(t.grad for t in leaves)])
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def _negated(t):
+    """t as the imaginary part of a conjugate, whose memory holds -t; dense where it is one value."""
+    v = torch.view_as_complex(torch.stack([t, -t], -1).contiguous()).conj().imag
+    assert v.is_neg() and torch.equal(v, t) and (t.numel() > 1 or v.is_contiguous())
+    return v
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 1), (5, 8)])
+def test_negated_views(shape):
+    x, r, dy = (torch.rand(*shape, device=DEV) + 1 for _ in range(3))
+    w = torch.rand(shape[1], device=DEV) + 1
+    for a, b in zip(rms_norm(_negated(x), _negated(w), 1.0, _negated(r)), rms_norm(x, w, 1.0, r)):
+        assert torch.equal(a, b)
+    for a, b in zip(rms_norm_int8(_negated(x), _negated(w), 1.0, _negated(r)), rms_norm_int8(x, w, 1.0, r)):
+        assert torch.equal(a, b)
+    for a, b in zip(quantize_rows(_negated(x)), quantize_rows(x)):
+        assert torch.equal(a, b)
+    q, s = quantize_rows(x)
+    assert torch.equal(int8_linear(q, _negated(s), q[:1], _negated(s[:1]), _negated(w[:1])), int8_linear(q, s, q[:1], s[:1], w[:1]))
+    got = []
+    for form in (_negated, lambda t: t):
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        y = rms_norm(form(leaves[0]), form(leaves[1]), 1.0)
+        y.backward(form(dy))
+        got.append([t.grad for t in leaves])
+        half = [t.half().requires_grad_() for t in (x, x[:1], w[:1])]
+        y = checkpointed_linear(*(form(t) for t in half), "silu")
+        y.backward(form(torch.ones_like(y)))
+        got[-1] += [y.detach(), *(t.grad for t in half)]
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

@@ -47,7 +47,8 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-Tensor contiguous(const Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+// (a negated view, the imaginary part of a conjugate, holds its values with the other sign: its memory is not read as it is)
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", nf_last_error()); }
 
@@ -61,9 +62,9 @@ struct Rows {
   Tensor hold;
   void* p;
   int64_t n, stride;
-  Rows(const Tensor& t, int64_t width) : hold(t), n(t.numel() / width), stride(width) {
-    if (!t.is_contiguous()) {
-      hold = t.reshape({-1, width});
+  Rows(const Tensor& t, int64_t width) : hold(t.resolve_neg()), n(t.numel() / width), stride(width) {
+    if (!hold.is_contiguous()) {
+      hold = hold.reshape({-1, width});
       if (hold.stride(1) != 1 || (n > 1 && hold.stride(0) < width)) hold = hold.contiguous();
       stride = hold.stride(0);
     }
