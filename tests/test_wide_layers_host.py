@@ -227,3 +227,17 @@ def test_alias_package_and_names():
         "norm.weight": (96,), "up.weight": (384, 96), "up.bias": (384,), "down.weight": (96, 384), "down.bias": (96,)}
     with pytest.raises(AssertionError, match="GPU"):
         m.to_int8()
+
+
+def test_leaves_on_the_host_with_a_graph_are_refused_as_such():
+    """Arguments are checked for their device, whatever else holds them."""
+    from triton_helpers_amd.layers.checkpointed_linear import checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm import rms_norm
+
+    x, w = torch.randn(4, 8).bfloat16().requires_grad_(), torch.ones(8).requires_grad_()
+    alive = x.float() * w
+    with pytest.raises(AssertionError, match="GPU"):
+        rms_norm(x, w)
+    with pytest.raises(AssertionError, match="GPU"):
+        checkpointed_linear(x, torch.randn(4, 8).bfloat16().requires_grad_(), w[:4])
+    del alive

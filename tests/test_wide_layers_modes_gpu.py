@@ -344,3 +344,39 @@ def test_negated_views(shape):
         got[-1] += [y.detach(), *(t.grad for t in half)]
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("mode", [False, True])
+@pytest.mark.parametrize("name", TRAINED)
+def test_a_capture_beside_an_eager_graph_is_refused(name, mode):
+    """Also where the Python Functions run (a default device is a mode): the forward refuses, while nothing has happened yet; afterwards the step replays."""
+    from contextlib import nullcontext
+
+    fn, args = operator(name)
+    leaves = [t.requires_grad_() for t in args]
+
+    def step():
+        with torch.device(DEV) if mode else nullcontext():
+            out = several(fn(*leaves))
+        return [*out, *torch.autograd.grad(out, leaves, [torch.ones_like(t) for t in out])]
+
+    alive = fn(*leaves)
+    with pytest.raises(RuntimeError, match="outside of this capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            with torch.device(DEV) if mode else nullcontext():
+                fn(*leaves)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), torch.no_grad():  # nothing to be refused: no gradient is asked for
+        with torch.device(DEV) if mode else nullcontext():
+            fn(*leaves)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(1, 4):
+        with torch.no_grad():
+            for t, v in zip(leaves, operator(name, seed)[1]):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)

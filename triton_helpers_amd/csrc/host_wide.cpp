@@ -9,7 +9,7 @@ namespace {
 // default stream, which cannot take part in a capture, a captured backward would end there: it has to wait for the captured stream, and torch ends the
 // process.  Refused in the forward, while nothing has happened yet.  (Any other stream joins the capture and is joined again.)
 void refuse_eager_graph(const Tensor& t) {
-  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
   if (node == nullptr || node->num_inputs() == 0) return;
   if (node->input_metadata(0).stream().id() != c10::hip::getDefaultHIPStream(t.device().index()).id() ||
@@ -17,6 +17,16 @@ void refuse_eager_graph(const Tensor& t) {
     return;
   TORCH_CHECK(false, "a graph that was built outside of this capture, on the default stream, still holds one of the leaves: delete what it computed (outputs, losses) before capturing a "
                      "step that takes gradients");
+}
+
+// refuse_eager_graphs(tensors or None ...): the same for the Python functions, in front of the autograd Functions that take over from here
+PyObject* refuse_eager_graphs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (at::GradMode::is_enabled())
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (THPVariable_Check(a[i])) refuse_eager_graph(THPVariable_Unpack(a[i]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
 }
 
 bool float_type(const Tensor& t) { return code_of(t.scalar_type()) >= 0; }
@@ -517,7 +527,7 @@ PyObject* checkpointed_linear_launch_backward(PyObject*, PyObject* const* a, Py_
 
 }  // namespace
 
-PyMethodDef wide_methods[] = {ENTRY(rms_norm), ENTRY(rms_norm_int8), ENTRY(rms_norm_launch_forward), ENTRY(rms_norm_launch_backward),
+PyMethodDef wide_methods[] = {ENTRY(refuse_eager_graphs), ENTRY(rms_norm), ENTRY(rms_norm_int8), ENTRY(rms_norm_launch_forward), ENTRY(rms_norm_launch_backward),
                               ENTRY(quantize_rows), ENTRY(quantize_rows_launch), ENTRY(int8_linear), ENTRY(int8_linear_launch),
                               ENTRY(checkpointed_linear), ENTRY(checkpointed_linear_launch_forward), ENTRY(checkpointed_linear_launch_backward),
                               {nullptr, nullptr, 0, nullptr}};

@@ -86,4 +86,5 @@ def checkpointed_linear(x: Tensor, w: Tensor, b: Optional[Tensor] = None, activa
     if y is not None:
         return y
     # a mode, a subclass, or arguments to be refused
+    _lib.native().refuse_eager_graphs(x, w, b)
     return _checkpointed_linear.apply(x, w, b, activation)

@@ -78,6 +78,7 @@ def rms_norm(x: Tensor, weight: Optional[Tensor], eps: float = 1e-6, residual: O
     if y is not None:
         return y
     # a mode, a subclass, or arguments to be refused
+    _lib.native().refuse_eager_graphs(x, weight, residual)
     return _rms_norm.apply(x, weight, eps, residual)
 
 
