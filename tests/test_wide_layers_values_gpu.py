@@ -41,3 +41,26 @@ def test_masked_rows_of_the_lowest_value(m, n, k, dtype, name):
     else:  # every gate is closed there
         assert not dw.any() and not dx[7].any()
     assert not dw[3:].any()
+
+
+def test_more_workgroups_than_one_row_of_a_grid_copies():
+    """Copies of more than 2^30 pieces of 16 bytes go to a grid of two dimensions, whose last workgroups have nothing to do.  dx alone, from a copied dy; dW, from act(x^) written out.
+    Whole numbers, and only the last rows have gradients: exact."""
+    m, tail = 2**23 + 3, 45
+    for n, k, need in ((1030, 8, "dx"), (8, 1030, "dw")):
+        g = torch.Generator(device=DEV).manual_seed(n)
+        w = torch.randint(-2, 3, (n, k), generator=g, device=DEV).bfloat16()
+        x, dy = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV), torch.zeros(m, n, dtype=torch.bfloat16, device=DEV)
+        x[-tail:] = torch.randint(-3, 4, (tail, k), generator=g, device=DEV).bfloat16()
+        x[-tail:, 1] = 127
+        dy[-tail:] = torch.randint(-2, 3, (tail, n), generator=g, device=DEV).bfloat16()
+        (x if need == "dx" else w).requires_grad_()
+        y = checkpointed_linear(x, w)
+        y.backward(dy)
+        if need == "dx":
+            want = (dy[-tail:].double() @ w.double()).bfloat16()
+            assert torch.equal(x.grad[-tail:], want) and not x.grad[:-tail].any() and w.grad is None
+        else:
+            assert torch.equal(w.grad, (dy[-tail:].double().t() @ x[-tail:].double()).bfloat16()) and x.grad is None
+        assert torch.equal(y[-tail:].detach(), (x[-tail:].detach().double() @ w.detach().double().t()).bfloat16()) and not y[:-tail].any()
+        del x, dy, w, y

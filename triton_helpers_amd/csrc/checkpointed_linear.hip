@@ -165,7 +165,7 @@ struct Prepare {
   const int8_t* q;
   const float* s;
   uint16_t* h;
-  int64_t rows;
+  int64_t rows, blocks;  // none of either: no act(x^) is wanted
   int width, act;
 };
 template <typename T, int J>
@@ -179,6 +179,7 @@ __global__ __launch_bounds__(256) void prepare_k(Prepare a) {
     }
     block -= a.copy[c].blocks;
   }
+  if (block >= a.blocks) return;  // (a grid of two dimensions holds some more than there are)
   const Cut<J> cut(block, (a.width + 7) / 8);
   int q[J][2];
   float scale[J];
@@ -386,7 +387,7 @@ int bwd(const KeepBwd& p, const void* dy, int64_t dys, const int8_t* q, const fl
   if (p.w_bytes > 0) copy(1, w, ws, n, k, packed_w);
   if (dw != nullptr) {
     make.q = q, make.s = scale, make.h = (uint16_t*)h, make.rows = rows, make.width = (int)k, make.act = act;
-    blocks += cut_blocks(rows * (p.ldk / 8), each);
+    blocks += make.blocks = cut_blocks(rows * (p.ldk / 8), each);
   }
   if (blocks > 0) {
     if (each == 1) hipLaunchKernelGGL((prepare_k<T, 1>), grid_of(blocks), dim3(256), 0, s, make);
