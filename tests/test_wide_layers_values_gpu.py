@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from triton_helpers_amd.layers.checkpointed_linear import checkpointed_linear
+from triton_helpers_amd.layers.wide_mlp import WideMLP
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -64,3 +65,20 @@ def test_more_workgroups_than_one_row_of_a_grid_copies():
             assert torch.equal(w.grad, (dy[-tail:].double().t() @ x[-tail:].double()).bfloat16()) and x.grad is None
         assert torch.equal(y[-tail:].detach(), (x[-tail:].detach().double() @ w.detach().double().t()).bfloat16()) and not y[:-tail].any()
         del x, dy, w, y
+
+
+@pytest.mark.parametrize("dtype,wide", [(torch.float16, False), (torch.float16, True), (torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, True)])
+def test_blocks_in_8_bits_follow_each_other(dtype, wide):
+    """The 8-bit forms of a network's blocks, each of its own type, with a residual stream of that type or of float32."""
+    torch.manual_seed(0)
+    first, second = (WideMLP(72, 136).to(DEV, dtype) for _ in range(2))
+    rows = torch.bfloat16 if dtype == torch.float32 else dtype
+    x, r = torch.randn(5, 72, device=DEV).to(rows), torch.randn(5, 72, device=DEV).to(torch.float32 if wide else rows)
+    out, stream = first.to_int8()(x, r)
+    assert out.dtype == rows and stream.dtype == r.dtype
+    out, stream = second.to_int8()(out, stream)
+    assert out.dtype == rows and stream.dtype == r.dtype and torch.isfinite(out).all()
+    want = [m.to_int8(rows) for m in (first, second)]
+    want = want[1](*want[0](x, r))
+    assert torch.equal(out, want[0]) and torch.equal(stream, want[1])
+    assert first.to_int8(torch.float32)(x, r)[0].dtype == torch.float32

@@ -32,8 +32,11 @@ class WideMLP(nn.Module):
         y, stream = (self.norm(x), x) if residual is None else self.norm(x, residual)
         return self.down(self.up(y)), stream
 
-    def to_int8(self, dtype: torch.dtype = torch.bfloat16) -> "Int8WideMLP":
-        """This block for inference, its weights rounded to 8 bits (on their GPU); results in ``dtype``."""
+    def to_int8(self, dtype: Optional[torch.dtype] = None) -> "Int8WideMLP":
+        """This block for inference, its weights rounded to 8 bits (on their GPU); results in ``dtype``, by default in the block's own type (in
+        bfloat16 where its parameters are float32), so that the next block takes them beside a residual of that type."""
+        if dtype is None:
+            dtype = torch.bfloat16 if self.up.weight.dtype == torch.float32 else self.up.weight.dtype
         return Int8WideMLP(self.norm.weight.detach().clone(), Int8Linear.from_linear(self.up, self.down.activation, dtype),
                            Int8Linear.from_linear(self.down, "none", dtype), self.norm.eps)
 
