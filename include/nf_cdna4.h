@@ -310,7 +310,8 @@ int nf_rms_norm_bwd(const void* dy, int64_t dy_stride, int x_dtype, const void* 
                     int64_t rows, int64_t width, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Rows as int8 with one float32 scale each: q = rint(x * (127 / a)), s = a / 127, a the largest magnitude of the row (as nf_rms_norm_fwd's 8-bit
- * rows).  q [rows, width] without gaps, or NULL where h alone is wanted.  h: NULL, or act(x) in x's type, rows h_stride values apart, h_stride the width or the next multiple
+ * rows).  q [rows, width] without gaps, or NULL where h alone is wanted.  h: NULL, or act(x) rounded to x's type (NF_ACT_RELU2 of float16:
+ * infinite from x = 256 on), rows h_stride values apart, h_stride the width or the next multiple
  * of 8 (the values in between become zeros). */
 int nf_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int8_t* q, float* scale, void* h, int64_t h_stride, int act, int64_t rows,
                      int64_t width, void* stream);
@@ -327,7 +328,7 @@ int nf_int8_linear(const int8_t* q, int64_t q_stride, const float* scale, const 
 /* A linear layer behind an activation that keeps its input as 8-bit rows for the backward, float16 or bfloat16 rows and weights.
  *   forward   y[m, n] = sum_k act(x[m, k]) w[n, k] + bias[n];  q, scale: the 8-bit rows of x (NULL both: nothing is kept)
  *   backward  x^ = scale q;  dx = (dy w) * act'(x^);  dw = dy^T act(x^);  db = column sums of dy; each written, each may be NULL
- * Sums in float32; act(x) and act(x^) enter the products rounded to the rows' type.  bias and db of any type, dw of the rows' type or float32.  dx and
+ * Sums in float32; act(x) and act(x^) enter the products rounded to the rows' type (NF_ACT_RELU2 of float16 rows: infinite from x = 256 on).  bias and db of any type, dw of the rows' type or float32.  dx and
  * q [rows, k] and dw [n, k] without gaps; y, q and dx on 16-byte boundaries, y's rows too where n is a multiple of 8.  Up to 2^29 rows and 2^20 channels
  * on either side.  Workspaces on 16-byte boundaries, sizes by the queries (with the call's own pointers and strides).  Results are the same bits on every run.  The backward wants at least one row; w may be NULL without dx, q and scale where
  * neither dw nor an activation's dx needs them. */

@@ -82,3 +82,29 @@ def test_blocks_in_8_bits_follow_each_other(dtype, wide):
     want = want[1](*want[0](x, r))
     assert torch.equal(out, want[0]) and torch.equal(stream, want[1])
     assert first.to_int8(torch.float32)(x, r)[0].dtype == torch.float32
+
+
+@pytest.mark.parametrize("m", [40, 4096])
+def test_relu2_at_the_end_of_float16(m):
+    """255.875^2 = 65472.0156 rounds to 65472, the last value but one; 256^2 leaves the type, and its row and column show it.  bfloat16 goes on."""
+    n, k = 24, 64
+    w = torch.full((n, k), 2.0**-10, device=DEV)
+    x = torch.zeros(m, k, device=DEV)
+    x[1, 3], x[2, 5], x[3] = 255.875, 256.0, -300.0
+    dy = torch.zeros(m, n, device=DEV)
+    dy[0], dy[1, 0], dy[2, 1] = 1.0, 2.0**-10, 2.0**-10
+    xl, wl = x.half().requires_grad_(), w.half().requires_grad_()
+    y = checkpointed_linear(xl, wl, None, "relu2")
+    y.backward(dy.half())
+    assert torch.equal(y[1].double(), torch.full((n,), 65472 / 1024, dtype=torch.float64, device=DEV).half().double())
+    assert torch.isinf(y[2]).all() and not y[0].any() and not y[3:].any()
+    # the 8-bit row of a single value is that value to float32's rounding (a / 127 * 127): the same 65472
+    assert torch.equal(wl.grad[0, 3], torch.tensor(65472 / 1024, device=DEV).half())
+    assert torch.isinf(wl.grad[1, 5]) and torch.isnan(wl.grad[2:, 5]).all()
+    rest = torch.ones(k, dtype=torch.bool, device=DEV)
+    rest[5] = False
+    assert torch.isfinite(wl.grad[:, rest]).all() and torch.isfinite(xl.grad).all()
+    xl, wl = x.bfloat16().requires_grad_(), w.bfloat16().requires_grad_()
+    y = checkpointed_linear(xl, wl, None, "relu2")
+    y.backward(dy.bfloat16())
+    assert torch.equal(y[2].double(), torch.full((n,), 64.0, dtype=torch.float64, device=DEV)) and torch.isfinite(wl.grad).all()

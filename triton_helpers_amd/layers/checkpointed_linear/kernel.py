@@ -14,6 +14,10 @@ so ``dx`` is exact without an activation, and the others carry the rounding to 8
 the value.  Gates that open at zero (``"relu"``, ``"relu2"``) see a value below half a step as zero, that is closed.  A row that holds
 an infinity or a NaN is NaN in ``x^``.
 
+``act(x)`` and ``act(x^)`` enter the products rounded to the tensors' 16-bit type, whose range they have to keep: ``"relu2"`` leaves that of float16
+from ``x = 256`` on, and the infinity goes on into the row's ``y``, into ``dW``'s column and, times a zero of ``dy``, into it as NaN.  bfloat16 has
+float32's range.
+
 float16 and bfloat16; under autocast float32 tensors are cast to its type, and the weight's gradient comes back as float32.
 """
 from __future__ import annotations
