@@ -83,15 +83,18 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& g, int id) {
 
 // The descriptor of `bytes` bytes from p on, and a load of 16 bytes a lane, 1 KB, straight to LDS: lane l's go to `to` + 16 l; a lane whose offset
 // leaves the descriptor's range gets zeros.  As assembly without outputs, because the compiler waits for every such load in front of a
-// transposing read; what waits is Gemm::wait_and_meet.  (M0 is the compiler's own scratch register, set right before each use.  Loads that the compiler does not count make its own waits longer, never shorter.)
+// transposing read; what waits is Gemm::wait_and_meet.  (Loads that the compiler does not count make its own waits longer, never shorter.)
 __device__ __forceinline__ i32x4_t buffer_of(const char* p, int bytes) {
   const uint64_t v = (uint64_t)(uintptr_t)p;
   return i32x4_t{__builtin_amdgcn_readfirstlane((int)(uint32_t)v), __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32) & 0xffff),
                  __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (M0 is a reserved register: nothing is allocated to it, but the compiler may hold a value of its own there)
 __device__ __forceinline__ void load_to_lds(i32x4_t buffer, int offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // One operand of a workgroup: R rows of C's side, and the loads that bring a step of it to LDS.
 //
