@@ -9,7 +9,7 @@
 // type for each value) is what the 16-bit matrix instructions take; sums stay in float32 and are rounded once.  Many rows of few channels have kernels of
 // their own that read each row once (checkpointed_narrow.hip).
 //
-// 16384 x 4096 x 4096 bf16 with GELU, forward and backward 1367 - 1405 us: 8-bit rows and act(x) 60, forward product 400 - 420, sums of dy's columns 42 + 5, act(x^) 50, dx 455 - 470
+// 16384 x 4096 x 4096 bf16 with GELU, forward and backward 1367 - 1445 us by the card; launched alone 8-bit rows and act(x) 60, forward product 400 - 420, sums of dy's columns 42 + 5, act(x^) 50, dx 455 - 470
 // (its gate, a GELU's slope of 2^26 values, takes 45 of it), dW 400 - 415.  Three products alone take 1230 at the forward's rate.
 #include "checkpointed_narrow.h"
 #include "gemm_tile.h"

@@ -6,7 +6,7 @@
 //             weights that sit in LDS, its gate, dx out; the workgroups' dW and db are added up afterwards, in a fixed order
 //
 // As separate passes (8-bit rows; act(x^); three products) the same bytes move two and a half times.  2^18 x 256 x 256 with ReLU, forward and backward:
-// 199 - 205 us instead of 353, of which the forward 85, the backward 117, the sums of 256 partial dW 12 and db 5 (launched alone some more); the least that has to move, 670 MB, takes 136 at a
+// 199 - 214 us by the card instead of 353, of which the forward 85, the backward 117, the sums of 256 partial dW 12 and db 5 (launched alone some more); the least that has to move, 670 MB, takes 136 at a
 // copy's rate.  The waves wait for memory and for each other: more under way (a third tile) costs registers that hold the weights, a tile of 64 rows (111 us the
 // forward) and four waves to a SIMD (162, spilled) were slower.
 //

@@ -9,7 +9,7 @@
 // all of the step is in registers, its two slots are free, and the next step has to be there.
 //
 // On tiles of 256 x 256: bf16 16384 x 4096 x 4096 along the sum 395 us alone, 408 - 425 in a training step (1290 - 1390 TFLOP/s), both operands crosswise 396 - 415;
-// int8 16384 x 8192 x 8192 820 us (2680 Tops/s).  The matrix units are busy for 70 % of the clocks (74 % crosswise, int8 69 %), at some 1.9 GHz; what
+// int8 16384 x 8192 x 8192 798 - 848 us by the card (2590 - 2760 Tops/s).  The matrix units are busy for 70 % of the clocks (74 % crosswise, int8 69 %), at some 1.9 GHz; what
 // bounds the rest is the loads: without them (their data stale) 1730 TFLOP/s.  Measured and not kept: matrix instructions of 32x32, 3 to 10 % slower; 64-byte steps
 // with a meeting every second one, 12 %; priorities for the waves that multiply, -4 to +7 %; groups of 2, 8 or 16 row tiles, up to 10 %.
 //

@@ -6,8 +6,8 @@
 //
 // Up to 64 rows the time is that of reading the weights once: int8_few_rows_k, no LDS for the operands, the summed dimension split over the waves of
 // a workgroup; 1 x 4096 x 16384 13.8 us (67 MB, 4.8 TB/s), 19 x 5000 x 4098 10.4 (1.9 TB/s: loads that start off 16 bytes, and three fifths of the chip).  Beyond, tiles on the 8-bit matrix instructions (gemm_tile.h); where the tiles are too few for the chip, the summed
-// dimension is split over workgroups, whose integer sums a second kernel adds up (integers: any order gives the same bits).  16384 x 8192 x 8192 820 us (2680
-// Tops/s), 2048 x 4096 x 4096 36 (1900: one round of small tiles, half of it on the way in and out).
+// dimension is split over workgroups, whose integer sums a second kernel adds up (integers: any order gives the same bits).  16384 x 8192 x 8192 798 - 848 us by
+// the card (2590 - 2760 Tops/s), 2048 x 4096 x 4096 35 - 38 (1810 - 1960: one round of small tiles, half of it on the way in and out).
 #include "gemm_tile.h"
 
 namespace nf {

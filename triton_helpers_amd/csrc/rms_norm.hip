@@ -10,7 +10,7 @@
 // residual in its place would cost a tensor of memory and a ninth of the traffic, and makes a 16-bit dw, whose own rounding is as large, 1.4 times as exact).
 //
 // 16384 x 4096 bf16 with a residual: forward 96 us (537 MB, 5.6 TB/s; a large copy reaches 4.9, part of this comes out of the memory-side cache), backward 127
-// and the sum of its dw 5 (4.2 TB/s); with autograd 229 a step.  5003 x 777 float32: 10.4, 12.5 and 4.2, and the host's 56 a step.  1 x 4096: 2.8, 6.3 a call.
+// and the sum of its dw 5 (4.2 TB/s); with autograd 229 a step.  5003 x 777 float32: 10.4, 12.5 and 4.2, and the host's 54 - 57 a step.  1 x 4096: 2.8, 6.2 - 6.4 a call.
 #include "wide_common.h"
 
 namespace nf {
