@@ -48,7 +48,9 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // (a negated view, the imaginary part of a conjugate, holds its values with the other sign: its memory is not read as it is)
-Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+Tensor contiguous(const Tensor& t) { return t.defined() ? resolved(t).contiguous() : t; }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", nf_last_error()); }
 
@@ -62,7 +64,7 @@ struct Rows {
   Tensor hold;
   void* p;
   int64_t n, stride;
-  Rows(const Tensor& t, int64_t width) : hold(t.resolve_neg()), n(t.numel() / width), stride(width) {
+  Rows(const Tensor& t, int64_t width) : hold(resolved(t)), n(t.numel() / width), stride(width) {
     if (!hold.is_contiguous()) {
       hold = hold.reshape({-1, width});
       if (hold.stride(1) != 1 || (n > 1 && hold.stride(0) < width)) hold = hold.contiguous();
