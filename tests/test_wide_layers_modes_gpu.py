@@ -380,3 +380,20 @@ def test_a_capture_beside_an_eager_graph_is_refused(name, mode):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+def test_python_functions_with_arguments_left_out():
+    from triton_helpers_amd.layers.checkpointed_linear.kernel import _checkpointed_linear
+    from triton_helpers_amd.layers.rms_norm.kernel import _rms_norm
+
+    x, w, b = (t.requires_grad_() for t in operator("checkpointed_linear")[1])
+    v = torch.rand(K, device=DEV).requires_grad_()
+    for short, full, leaves in ((lambda: _checkpointed_linear.apply(x, w), lambda: checkpointed_linear(x, w), (x, w)),
+                                (lambda: _checkpointed_linear.apply(x, w, b), lambda: checkpointed_linear(x, w, b), (x, w, b)),
+                                (lambda: _rms_norm.apply(x, v), lambda: rms_norm(x, v), (x, v)),
+                                (lambda: _rms_norm.apply(x, v, 0.5), lambda: rms_norm(x, v, 0.5), (x, v)),
+                                (lambda: _rms_norm.apply(x, None), lambda: rms_norm(x, None), (x,))):
+        got, want = short(), full()
+        assert torch.equal(got, want)
+        for a, c in zip(torch.autograd.grad(got.float().square().sum(), leaves), torch.autograd.grad(want.float().square().sum(), leaves)):
+            assert torch.equal(a, c)

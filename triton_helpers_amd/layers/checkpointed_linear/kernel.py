@@ -56,7 +56,7 @@ def _validate(x: Tensor, w: Tensor, b: Optional[Tensor], activation: str) -> Non
 
 class _checkpointed_linear(Function):
     @staticmethod
-    def forward(ctx, x: Tensor, w: Tensor, b: Optional[Tensor], activation: str = "none") -> Tensor:
+    def forward(ctx, x: Tensor, w: Tensor, b: Optional[Tensor] = None, activation: str = "none") -> Tensor:
         _validate(x, w, b, activation)
         ctx.float_dw = w.dtype == torch.float32
         ctx.x_dtype = x.dtype
@@ -71,7 +71,7 @@ class _checkpointed_linear(Function):
 
     @staticmethod
     def backward(ctx, dy: Tensor):
-        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
+        need_dx, need_dw, need_db = (*ctx.needs_input_grad, False)[:3]  # (the bias may have been left out)
         dx, dw, db = _lib.native().checkpointed_linear_launch_backward(
             *ctx.saved_tensors, _lib.NF_ACT[ctx.activation], dy, need_dx, need_dw, need_db, ctx.float_dw, ctx.b_code)
         return None if dx is None else dx.to(ctx.x_dtype), dw, db, None

@@ -50,7 +50,7 @@ class _rms_norm(Function):
     @staticmethod
     def backward(ctx, dy: Optional[Tensor], d_residual: Optional[Tensor] = None):
         h, rstd, weight = ctx.saved_tensors
-        need_x, need_w, _, need_r = ctx.needs_input_grad
+        need_x, need_w, _, need_r = (*ctx.needs_input_grad, False, False)[:4]  # (eps and the residual may have been left out)
         dx, dw, dr = _lib.native().rms_norm_launch_backward(h, rstd, weight, ctx.like, dy, d_residual, ctx.residual, need_x or need_r, need_w)
         return dx, dw, None, dr
 
